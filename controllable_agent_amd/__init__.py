@@ -8,7 +8,7 @@ Compute goes through libfbhip.so (hand-written HIP kernels, include/fbhip.h); th
 from ._lib import LIB_PATH  # noqa: F401
 
 __all__ = ["FBHipAgent", "FBDDPGAgentConfig", "DiscreteFBHipAgent", "DiscreteFBAgentConfig", "SFHipAgent", "SFAgentConfig",
-           "DeviceReplayBuffer", "EpisodeBatch", "kernels"]
+           "DeviceReplayBuffer", "EpisodeBatch", "AdamW", "kernels"]
 
 
 def __getattr__(name):
@@ -18,6 +18,9 @@ def __getattr__(name):
     if name in ("DeviceReplayBuffer", "EpisodeBatch"):
         from . import replay
         return getattr(replay, name)
+    if name == "AdamW":
+        from .adamw import AdamW
+        return AdamW
     if name == "kernels":
         import importlib
         return importlib.import_module(".kernels", __name__)

@@ -126,6 +126,9 @@ PROTOTYPES = {
     "fbhip_pairwise_fb_block": (C.c_int, [_P] * 7 + [_I, _I, _I, _F, _I, _I] + [_P] * 5 + [_P]),
     "fbhip_adam_ema": (C.c_int, [_P, _P, _P, _P, _P, _L, _F, _I, _F, _F, _P]),
     "fbhip_inverse": (C.c_int, [_P, _I, _I, _F, _P, _I, _P]),
+    "fbhip_adamw_partials": (_I, [_I]),
+    "fbhip_adamw_set_step": (C.c_int, [_P, _L, _P]),
+    "fbhip_adamw_step": (C.c_int, [_P, _P, _P, _P, C.c_double, _F, _I, _F, _P]),
 }
 
 _lib = None

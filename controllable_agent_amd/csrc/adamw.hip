@@ -1,0 +1,397 @@
+// One AdamW step over many tensors in one launch, moments in 32 or in 8 bits, and the global gradient norm that clips it.
+//
+//   g = gs * grad                          gs = grad_scale * min(1, max_norm / norm),  norm = |grad_scale| sqrt(sum of all grad^2)
+//   m <- m + (1-b1)(g - m);   v <- b2 v + (1-b2) g g
+//   p <- (1 - lr wd) p - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps)
+//
+// Bound by HBM: 28 bytes an element with fp32 parameters, gradients and moments, 16 with 8-bit moments.  Every stream is read once and
+// written once; a lane holds eight consecutive elements, so that each 16-bit stream is one 16-byte access, an fp32 one two and a code
+// stream one of 8 bytes, and a block of 256 elements that shares a scale is half a wave: its maximum is five lane exchanges.
+//
+// 8-bit moments.  m and r = sqrt(v) are held as e4m3 codes times a power of two for each 256 elements (the least one under which the
+// block's largest magnitude is at most 448).  r, not v: the step divides by sqrt(v), and the root halves the range that the codes have to
+// span.  Codes are rounded up or down at random so that their mean is the value: a step moves v by a thousandth (1 - b2), half a code step
+// is 3 %, and nearest rounding would never move r at all.  A positive r never rounds to zero (the update would divide by eps alone).
+// The arithmetic before the codes is written without contraction, so that a code depends on single-precision operations in the order of
+// the formulas and on nothing else.  A value that is no number keeps its own code (NaN) and does not touch the block's scale.
+#include "common.h"
+#include "fbhip.h"
+
+#include <cmath>
+
+namespace fbhip {
+
+constexpr int ADAMW_THREADS = 256, ADAMW_PER_LANE = 8, ADAMW_CHUNK = ADAMW_THREADS * ADAMW_PER_LANE;
+static_assert(ADAMW_CHUNK == FBHIP_ADAMW_CHUNK, "the caller's chunk table counts chunks of this size");
+constexpr int ADAMW_MAX_TENSORS = 384;       // gradient addresses travel in the kernel arguments (4 KB): valid in a captured graph
+constexpr int ADAMW_BLOCKS = 2048;           // eight workgroups for each of 256 CUs; they walk the chunks
+constexpr int ADAMW_NORM_BLOCKS = 1024;      // one partial sum each, folded in order
+
+// The optimiser's scalars on the device (FBHIP_ADAMW_CONTROL_BYTES): a replayed graph advances them.
+struct AdamwControl {
+    int64_t t;                               // steps done
+    double b1t, b2t;                         // b1^t, b2^t
+    float norm, gs;                          // of this step, where it clips
+    int32_t skip;                            // the norm is not finite: the step changes nothing
+    uint32_t step_ticket, norm_ticket;
+};
+static_assert(sizeof(AdamwControl) <= FBHIP_ADAMW_CONTROL_BYTES, "control block");
+
+struct AdamwArgs {
+    const fbhip_adamw_tensor* tensors;
+    const int2* chunks;                      // (tensor, chunk of it)
+    int first, last;                         // chunks of this launch
+    int tensor0;                             // grad[] starts at this tensor
+    int advance;                             // this launch is the step's last one
+    int clip;
+    AdamwControl* ctl;
+    void *m, *v;                             // float, or codes
+    float *m_scale, *r_scale;
+    double lr, b1, b2;
+    const float* lr_ptr;
+    float eps, grad_scale;
+    uint32_t seed;
+    const void* grad[ADAMW_MAX_TENSORS];
+    uint8_t gtype[ADAMW_MAX_TENSORS];
+};
+static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
+
+struct NormArgs {
+    const fbhip_adamw_tensor* tensors;
+    const int2* chunks;
+    int first, last, tensor0;
+    int partial0, partials;                  // this launch's first partial sum, and how many there are in the last launch (else 0)
+    double* partial;
+    AdamwControl* ctl;
+    float max_norm, grad_scale;
+    const void* grad[ADAMW_MAX_TENSORS];
+    uint8_t gtype[ADAMW_MAX_TENSORS];
+};
+static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ float bf16_float(uint32_t h) { return __uint_as_float(h << 16); }
+__device__ __forceinline__ float fp16_float(uint16_t h) { _Float16 x; __builtin_memcpy(&x, &h, 2); return (float)x; }
+
+__device__ __forceinline__ float load_one(const void* base, int64_t i, int type) {
+    if (type == FBHIP_F32) return ((const float*)base)[i];
+    const uint16_t h = ((const uint16_t*)base)[i];
+    return type == FBHIP_BF16 ? bf16_float(h) : fp16_float(h);
+}
+
+// eight consecutive elements from a 16-byte aligned address
+__device__ __forceinline__ void load_eight(const void* base, int64_t i, int type, float (&x)[8]) {
+    if (type == FBHIP_F32) {
+        const float4 a = *(const float4*)((const float*)base + i), b = *(const float4*)((const float*)base + i + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        return;
+    }
+    const uint4 q = *(const uint4*)((const uint16_t*)base + i);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = type == FBHIP_BF16 ? bf16_float(w[j] & 0xFFFFu) : fp16_float((uint16_t)w[j]);
+        x[2 * j + 1] = type == FBHIP_BF16 ? __uint_as_float(w[j] & 0xFFFF0000u) : fp16_float((uint16_t)(w[j] >> 16));
+    }
+}
+
+// Where element i of a tensor lies: dense tensors are one run in storage order; a row-strided matrix has its own leading dimension.
+struct Walk {
+    int64_t row; int col, cols, ld;
+    __device__ __forceinline__ Walk(int64_t i, int cols_, int ld_) : cols(cols_), ld(ld_) { row = i / cols_; col = (int)(i - row * cols_); }
+    __device__ __forceinline__ int64_t at() const { return row * ld + col; }
+    __device__ __forceinline__ void next() { if (++col == cols) { col = 0; ++row; } }
+};
+
+// The gradient's eight elements from i on (zero behind the tensor's end).
+__device__ __forceinline__ void load_grad(const fbhip_adamw_tensor& T, const void* g, int gtype, int64_t i, float (&x)[8]) {
+    const bool flat = T.cols == 0 || (gtype & FBHIP_GRAD_DENSE);
+    gtype &= FBHIP_GRAD_DENSE - 1;
+    if (flat && i + 8 <= T.numel && ((uintptr_t)g & 15) == 0) { load_eight(g, i, gtype, x); return; }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    if (i >= T.numel) return;
+    if (flat) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (i + j < T.numel) x[j] = load_one(g, i + j, gtype);
+    } else {
+        Walk w(i, T.cols, T.ld);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { if (i + j < T.numel) x[j] = load_one(g, w.at(), gtype); w.next(); }
+    }
+}
+
+// A 32-bit word for an element: its place is multiplied and shifted into the step's key (two rounds of multiply and shift-xor).
+__device__ __forceinline__ uint32_t finish_word(uint32_t h) {
+    h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
+    h = (h ^ (h >> 13)) * 0xC2B2AE35u;
+    return h ^ (h >> 16);
+}
+__device__ __forceinline__ uint32_t element_word(int64_t i, uint32_t key) {
+    // places beyond 2^32 take a key of their own
+    return finish_word((uint32_t)i * 0x9E3779B1u + key + (uint32_t)((uint64_t)i >> 32) * 0x27D4EB2Fu);
+}
+
+// e4m3 codes of eight lane values and the block's scale (half a wave = 256 elements); u: 16 random bits for each value
+template <bool POSITIVE>
+__device__ __forceinline__ uint2 encode_eight(const float (&x)[8], const uint32_t (&u)[8], float& scale) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+        top = max(top, b < 0x7F800000u ? b : 0u);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    // 448 = 1.75 * 2^8: the exponent field of 2^k with top * 2^-k <= 448; at least 1, so that 2^k and 2^-k are normal numbers
+    const int field = max((int)((top + 0x1FFFFFu) >> 23) - 8, 1);
+    scale = __uint_as_float((uint32_t)field << 23);
+    const float inv = __uint_as_float((uint32_t)(254 - field) << 23);
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __float_as_uint(x[j]), mag = b & 0x7FFFFFFFu;
+        const float y = __uint_as_float(mag) * inv;
+        // three mantissa bits stay; below 2^-6 the codes are evenly spaced, which adding 2^-6 brings about
+        const bool small = y < 0.015625f;
+        const uint32_t z = __float_as_uint(small ? y + 0.015625f : y);
+        int code = (int)((z + (u[j] << 4)) >> 20) - (small ? 968 : 960);
+        if (POSITIVE) code = (code == 0 && mag != 0) ? 1 : code;
+        code = mag < 0x7F800000u ? code : 0x7F;
+        c[j] = (uint32_t)code | (POSITIVE ? 0u : (b >> 24) & 0x80u);
+    }
+    return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+}
+
+__device__ __forceinline__ void decode_eight(uint2 q, float scale, float (&x)[8]) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
+    const auto c = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
+    x[0] = a[0] * scale; x[1] = a[1] * scale; x[2] = b[0] * scale; x[3] = b[1] * scale;
+    x[4] = c[0] * scale; x[5] = c[1] * scale; x[6] = d[0] * scale; x[7] = d[1] * scale;
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a) {
+#pragma clang fp contract(off)
+    __shared__ double shared_lr, shared_ibc1;
+    __shared__ float shared_rbc2, shared_gs;
+    __shared__ uint32_t shared_key;
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        const AdamwControl c = *a.ctl;
+        const double b1t = c.b1t * a.b1, b2t = c.b2t * a.b2;
+        shared_lr = a.lr_ptr != nullptr ? (double)*a.lr_ptr : a.lr;
+        shared_ibc1 = 1.0 / (1.0 - b1t);
+        shared_rbc2 = (float)(1.0 / sqrt(1.0 - b2t));
+        shared_gs = a.clip ? c.gs : a.grad_scale;
+        shared_key = finish_word(a.seed ^ (uint32_t)(c.t + 1) * 0x27D4EB2Fu);
+        const bool skip = a.clip && c.skip;
+        if (skip) shared_gs = __uint_as_float(0x7FC00000u);
+        if (a.advance && !skip) {
+            // every workgroup has read the scalars when the last one comes here: it moves them to the next step
+            if (__hip_atomic_fetch_add(&a.ctl->step_ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
+                a.ctl->step_ticket = 0;
+                a.ctl->t = c.t + 1;
+                a.ctl->b1t = b1t;
+                a.ctl->b2t = b2t;
+            }
+        }
+    }
+    __syncthreads();
+    const float gs = shared_gs, rbc2 = shared_rbc2, eps = a.eps;
+    if (a.clip && gs != gs) return;
+    const double lr = shared_lr, ibc1 = shared_ibc1;
+    const uint32_t key = shared_key;
+    const float w1 = (float)(1.0 - a.b1), w2 = (float)(1.0 - a.b2), b2 = (float)a.b2;
+    for (int c = a.first + (int)blockIdx.x; c < a.last; c += (int)gridDim.x) {
+        const int2 e = a.chunks[c];
+        const fbhip_adamw_tensor T = a.tensors[e.x];
+        const int64_t i = (int64_t)e.y * ADAMW_CHUNK + tid * ADAMW_PER_LANE;
+        // the moments are padded to whole blocks of 256 for each tensor: half a wave is inside or outside as one
+        if (i >= ((T.numel + 255) & ~(int64_t)255)) continue;
+        const int64_t s = T.at + i;
+        float g[8], p[8], m[8], v[8];
+        load_grad(T, a.grad[e.x - a.tensor0], a.gtype[e.x - a.tensor0], i, g);
+        const bool whole = T.cols == 0 && i + 8 <= T.numel && ((uintptr_t)T.p & 15) == 0;
+        if (whole) load_eight(T.p, i, T.dtype, p);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = 0.f;
+            if (T.cols == 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (i + j < T.numel) p[j] = load_one(T.p, i + j, T.dtype);
+            } else {
+                Walk w(i, T.cols, T.ld);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { if (i + j < T.numel) p[j] = load_one(T.p, w.at(), T.dtype); w.next(); }
+            }
+        }
+        if (BITS == 32) {
+            load_eight(a.m, s, FBHIP_F32, m);
+            load_eight(a.v, s, FBHIP_F32, v);
+        } else {
+            const uint2 qm = *(const uint2*)((const uint8_t*)a.m + s), qr = *(const uint2*)((const uint8_t*)a.v + s);
+            decode_eight(qm, a.m_scale[s >> 8], m);
+            decode_eight(qr, a.r_scale[s >> 8], v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = v[j] * v[j];
+        }
+        const double lrt = lr * T.lr_scale;
+        const float keep = (float)(1.0 - lrt * T.weight_decay), ss = (float)(lrt * ibc1);
+        float r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float gr = g[j] * gs;
+            m[j] = m[j] + w1 * (gr - m[j]);
+            v[j] = v[j] * b2 + (w2 * gr) * gr;
+            r[j] = sqrtf(v[j]);
+            const float den = r[j] * rbc2 + eps;
+            p[j] = p[j] * keep - ss * (m[j] / den);
+        }
+        uint32_t word[8];
+        if (BITS == 8 || T.dtype == FBHIP_BF16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) word[j] = element_word(s + j, key);
+        }
+        if (BITS == 32) {
+            *(float4*)((float*)a.m + s) = make_float4(m[0], m[1], m[2], m[3]);
+            *(float4*)((float*)a.m + s + 4) = make_float4(m[4], m[5], m[6], m[7]);
+            *(float4*)((float*)a.v + s) = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4*)((float*)a.v + s + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint32_t u[8];
+            float scale;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = word[j] >> 16;
+            *(uint2*)((uint8_t*)a.m + s) = encode_eight<false>(m, u, scale);
+            if ((tid & 31) == 0) a.m_scale[s >> 8] = scale;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = word[j] & 0xFFFFu;
+            *(uint2*)((uint8_t*)a.v + s) = encode_eight<true>(r, u, scale);
+            if ((tid & 31) == 0) a.r_scale[s >> 8] = scale;
+        }
+        if (T.dtype == FBHIP_BF16) {
+            // up or down at random: bf16 steps are 0.4 % apart, and an update of a thousandth of that still has to count on average
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = __float_as_uint(p[j]);
+                h[j] = p[j] != p[j] ? 0x7FC0u : (b + (word[j] * 0x9E3779B1u >> 16)) >> 16;
+            }
+            if (whole) {
+                *(uint4*)((uint16_t*)T.p + i) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            } else if (i < T.numel) {
+                Walk w(i, T.cols == 0 ? 0x7FFFFFFF : T.cols, T.ld);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (i + j < T.numel) ((uint16_t*)T.p)[T.cols == 0 ? i + j : w.at()] = (uint16_t)h[j];
+                    w.next();
+                }
+            }
+        } else if (whole) {
+            *(float4*)((float*)T.p + i) = make_float4(p[0], p[1], p[2], p[3]);
+            *(float4*)((float*)T.p + i + 4) = make_float4(p[4], p[5], p[6], p[7]);
+        } else if (i < T.numel) {
+            Walk w(i, T.cols == 0 ? 0x7FFFFFFF : T.cols, T.ld);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (i + j < T.numel) ((float*)T.p)[T.cols == 0 ? i + j : w.at()] = p[j];
+                w.next();
+            }
+        }
+    }
+}
+
+// sum of squares in doubles (the square of the largest fp32 is far inside their range), lanes folded in a fixed tree
+__device__ __forceinline__ double block_sum(double x, double* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+__global__ void __launch_bounds__(ADAMW_THREADS) adamw_norm_kernel(const NormArgs a) {
+    __shared__ double red[4], red2[4];
+    __shared__ int is_last;
+    const int tid = threadIdx.x;
+    double acc = 0.0;
+    for (int c = a.first + (int)blockIdx.x; c < a.last; c += (int)gridDim.x) {
+        const int2 e = a.chunks[c];
+        const fbhip_adamw_tensor T = a.tensors[e.x];
+        float g[8];
+        load_grad(T, a.grad[e.x - a.tensor0], a.gtype[e.x - a.tensor0], (int64_t)e.y * ADAMW_CHUNK + tid * ADAMW_PER_LANE, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc += (double)g[j] * (double)g[j];
+    }
+    const double sum = block_sum(acc, red);
+    if (tid == 0) {
+        __hip_atomic_store(a.partial + a.partial0 + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        is_last = a.partials > 0 &&
+                  __hip_atomic_fetch_add(&a.ctl->norm_ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!is_last) return;
+    double x = 0.0;
+    for (int k = tid; k < a.partials; k += ADAMW_THREADS)
+        x += __hip_atomic_load(a.partial + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double total = block_sum(x, red2);
+    if (tid != 0) return;
+    const float norm = (float)(fabs((double)a.grad_scale) * sqrt(total));
+    const bool finite = norm < __uint_as_float(0x7F800000u);
+    a.ctl->norm_ticket = 0;
+    a.ctl->norm = norm;
+    a.ctl->skip = finite ? 0 : 1;
+    a.ctl->gs = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.f);
+}
+
+__global__ void adamw_set_kernel(AdamwControl* c, int64_t t, double b1t, double b2t) {
+    c->t = t; c->b1t = b1t; c->b2t = b2t;
+    c->norm = 0.f; c->gs = 1.f; c->skip = 0;
+    c->step_ticket = 0; c->norm_ticket = 0;
+}
+
+hipError_t launch_adamw_set(void* control, int64_t t, double b1, double b2, hipStream_t s) {
+    hipLaunchKernelGGL(adamw_set_kernel, dim3(1), dim3(1), 0, s, (AdamwControl*)control, t, std::pow(b1, (double)t), std::pow(b2, (double)t));
+    return hipGetLastError();
+}
+
+hipError_t launch_adamw_step(const fbhip_adamw* o, const void* const* grads, const uint8_t* gtypes, const float* lr_ptr, double lr,
+                             float grad_scale, int clip, float max_norm, hipStream_t s) {
+    const int n = o->n_tensors, launches = (n + ADAMW_MAX_TENSORS - 1) / ADAMW_MAX_TENSORS;
+    if (clip) {
+        NormArgs a{};
+        a.tensors = o->tensors; a.chunks = (const int2*)o->chunks;
+        a.partial = o->partials; a.ctl = (AdamwControl*)o->control;
+        a.max_norm = max_norm; a.grad_scale = grad_scale;
+        int done = 0;
+        for (int l = 0; l < launches; ++l) {
+            const int t0 = l * ADAMW_MAX_TENSORS, t1 = min(n, t0 + ADAMW_MAX_TENSORS);
+            a.first = o->host_first_chunk[t0]; a.last = o->host_first_chunk[t1]; a.tensor0 = t0;
+            for (int t = t0; t < t1; ++t) { a.grad[t - t0] = grads[t]; a.gtype[t - t0] = gtypes[t]; }
+            const int blocks = max(1, min(ADAMW_NORM_BLOCKS, a.last - a.first));
+            a.partial0 = done;
+            done += blocks;
+            a.partials = l == launches - 1 ? done : 0;
+            hipLaunchKernelGGL(adamw_norm_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, s, a);
+        }
+    }
+    AdamwArgs a{};
+    a.tensors = o->tensors; a.chunks = (const int2*)o->chunks; a.ctl = (AdamwControl*)o->control; a.clip = clip;
+    a.m = o->m; a.v = o->v; a.m_scale = o->m_scale; a.r_scale = o->r_scale;
+    a.lr = lr; a.lr_ptr = lr_ptr; a.b1 = o->beta1; a.b2 = o->beta2; a.eps = o->eps; a.grad_scale = grad_scale; a.seed = o->seed;
+    for (int l = 0; l < launches; ++l) {
+        const int t0 = l * ADAMW_MAX_TENSORS, t1 = min(n, t0 + ADAMW_MAX_TENSORS);
+        a.first = o->host_first_chunk[t0]; a.last = o->host_first_chunk[t1]; a.tensor0 = t0;
+        a.advance = l == launches - 1;
+        for (int t = t0; t < t1; ++t) { a.grad[t - t0] = grads[t]; a.gtype[t - t0] = gtypes[t]; }
+        const int blocks = max(1, min(ADAMW_BLOCKS, a.last - a.first));
+        if (o->bits == 32) hipLaunchKernelGGL(adamw_kernel<32>, dim3(blocks), dim3(ADAMW_THREADS), 0, s, a);
+        else hipLaunchKernelGGL(adamw_kernel<8>, dim3(blocks), dim3(ADAMW_THREADS), 0, s, a);
+    }
+    return hipGetLastError();
+}
+
+int adamw_partials(int n_tensors) { return (n_tensors + ADAMW_MAX_TENSORS - 1) / ADAMW_MAX_TENSORS * ADAMW_NORM_BLOCKS; }
+
+}  // namespace fbhip
+

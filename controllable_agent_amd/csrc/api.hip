@@ -1334,5 +1334,40 @@ int fbhip_actor_head_bwd(const float* dt1, int32_t ldt, const float* lnY, const 
     return FBHIP_OK;
 }
 
-}  // extern "C"
+// ---- AdamW over many tensors -----------------------------------------------------------------------------------
+int32_t fbhip_adamw_partials(int32_t n_tensors) { return n_tensors < 1 ? 0 : adamw_partials(n_tensors); }
 
+static int check_adamw(const fbhip_adamw* o) {
+    if (o == nullptr || o->struct_size != sizeof(fbhip_adamw)) { g_err = "fbhip_adamw: struct_size does not match this library"; return FBHIP_E_INVALID; }
+    if (o->n_tensors < 1 || !o->tensors || !o->chunks || !o->host_first_chunk || !o->m || !o->v || !o->control ||
+        (o->bits != 8 && o->bits != 32) || (o->bits == 8 && (!o->m_scale || !o->r_scale))) {
+        g_err = "fbhip_adamw: a table, a moment array or the control block is missing, or bits is neither 8 nor 32"; return FBHIP_E_INVALID;
+    }
+    if (!(o->beta1 >= 0 && o->beta1 < 1 && o->beta2 >= 0 && o->beta2 < 1 && o->eps >= 0)) { g_err = "fbhip_adamw: 0 <= beta < 1, eps >= 0"; return FBHIP_E_INVALID; }
+    return FBHIP_OK;
+}
+
+int fbhip_adamw_set_step(const fbhip_adamw* opt, int64_t step, void* stream) {
+    fbhip_ctx* none = nullptr;
+    RC(check_adamw(opt));
+    if (step < 0) { g_err = "fbhip_adamw_set_step: step >= 0"; return FBHIP_E_INVALID; }
+    HIPCK(none, launch_adamw_set(opt->control, step, opt->beta1, opt->beta2, (hipStream_t)stream));
+    return FBHIP_OK;
+}
+
+int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, const uint8_t* host_grad_types, const float* lr_device,
+                     double lr, float grad_scale, int32_t clip, float max_norm, void* stream) {
+    fbhip_ctx* none = nullptr;
+    RC(check_adamw(opt));
+    if (!host_grads || !host_grad_types) { g_err = "fbhip_adamw_step: gradients required"; return FBHIP_E_INVALID; }
+    if (clip && (!opt->partials || !(max_norm > 0))) { g_err = "fbhip_adamw_step: clipping needs partials and max_norm > 0"; return FBHIP_E_INVALID; }
+    for (int t = 0; t < opt->n_tensors; ++t) {
+        if (opt->host_first_chunk[t] > opt->host_first_chunk[t + 1]) { g_err = "fbhip_adamw_step: chunk table not ascending"; return FBHIP_E_INVALID; }
+        if (!host_grads[t] && opt->host_first_chunk[t] < opt->host_first_chunk[t + 1]) { g_err = "fbhip_adamw_step: a gradient is missing"; return FBHIP_E_INVALID; }
+        if ((host_grad_types[t] & ~FBHIP_GRAD_DENSE) > FBHIP_F16) { g_err = "fbhip_adamw_step: unknown gradient type"; return FBHIP_E_INVALID; }
+    }
+    HIPCK(none, launch_adamw_step(opt, host_grads, host_grad_types, lr_device, lr, grad_scale, clip, max_norm, (hipStream_t)stream));
+    return FBHIP_OK;
+}
+
+}  // extern "C"

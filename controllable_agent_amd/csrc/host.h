@@ -195,6 +195,12 @@ struct fbhip_ctx {
     } while (0)
 
 namespace fbhip {
+// ---- AdamW over many tensors (adamw.hip)
+int adamw_partials(int n_tensors);
+hipError_t launch_adamw_set(void* control, int64_t t, double b1, double b2, hipStream_t s);
+hipError_t launch_adamw_step(const fbhip_adamw* o, const void* const* grads, const uint8_t* gtypes, const float* lr_ptr, double lr,
+                             float grad_scale, int clip, float max_norm, hipStream_t s);
+
 namespace host {
 
 // ------------------------------------------------------------------------------------------------ schedule (schedule.hip)

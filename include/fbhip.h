@@ -22,7 +22,7 @@
  *     ``fbhip_read_metrics``), and launches everything asynchronously on the caller's stream;
  *   - every function returns 0 on success or a negative FBHIP_E_* code; the message is available from
  *     ``fbhip_last_error``; nothing is ever thrown across the ABI;
- *   - all matrices are float32 row-major with an explicit leading dimension (in floats).
+ *   - all matrices are float32 row-major with an explicit leading dimension (in floats), unless an entry point names other types.
  */
 #ifndef FBHIP_H
 #define FBHIP_H
@@ -470,6 +470,51 @@ int fbhip_adam_ema(float* params, const float* grads, float* m, float* v, float*
 /* out[d,d] = inverse(scale * A[d,d]), 1 <= d <= 128: Gauss-Jordan with partial pivoting in fp64 on one workgroup -- torch.inverse of
  * the q_loss covariance (fb_ddpg.py:334-335) and the pinv of SFAgent's z-mix covariance (sf.py:731-732, full rank). */
 int fbhip_inverse(const float* A, int32_t lda, int32_t d, float scale, float* out, int32_t ldo, void* stream);
+
+/* ---- AdamW over many tensors (csrc/adamw.hip) ------------------------------------------------------- */
+/* element types of operands that are not all float32 */
+enum { FBHIP_F32 = 0, FBHIP_BF16 = 1, FBHIP_F16 = 2 };
+#define FBHIP_GRAD_DENSE 4                 /* gradient type flag: the gradient of a row-strided parameter is itself dense */
+#define FBHIP_ADAMW_CHUNK 2048             /* elements of a tensor that one workgroup takes at a time */
+#define FBHIP_ADAMW_CONTROL_BYTES 64
+/* One parameter, in DEVICE memory.  cols == 0: one dense run of numel elements (in storage order); cols > 0: a row-major matrix of
+ * numel / cols rows with leading dimension ld >= cols.  at: its first element in the moment arrays, a multiple of 256. */
+typedef struct fbhip_adamw_tensor {
+    void* p;
+    int64_t numel;
+    int64_t at;
+    int32_t cols, ld;
+    double weight_decay;
+    double lr_scale;                       /* the tensor's learning rate is lr * lr_scale */
+    int32_t dtype;                         /* FBHIP_F32 or FBHIP_BF16 */
+    int32_t reserved;
+} fbhip_adamw_tensor;
+typedef struct fbhip_adamw {
+    uint32_t struct_size;                  /* sizeof(fbhip_adamw) */
+    int32_t n_tensors;
+    const fbhip_adamw_tensor* tensors;     /* [n_tensors] */
+    const int32_t* chunks;                 /* [n_chunks][2]: (tensor, which chunk of it), tensors ascending */
+    const int32_t* host_first_chunk;       /* HOST [n_tensors + 1]: first chunk of each tensor, and n_chunks */
+    int32_t bits;                          /* 32: m, v float32; 8: m and r = sqrt(v) as e4m3 codes, m_scale / r_scale per 256 elements */
+    uint32_t seed;                         /* of the random bits that 8-bit moments and bfloat16 parameters are rounded with */
+    void* m;
+    void* v;
+    float* m_scale;
+    float* r_scale;
+    void* control;                         /* FBHIP_ADAMW_CONTROL_BYTES: step count, gradient norm (float at byte 24) */
+    double* partials;                      /* fbhip_adamw_partials doubles; nullable where no step clips */
+    double beta1, beta2;
+    float eps;
+} fbhip_adamw;
+/* doubles that clipping needs for n_tensors */
+int32_t fbhip_adamw_partials(int32_t n_tensors);
+/* sets the step count (steps already done) */
+int fbhip_adamw_set_step(const fbhip_adamw* opt, int64_t step, void* stream);
+/* One step.  host_grads: HOST array of n_tensors device pointers; host_grad_types: their FBHIP_F32 / BF16 / F16, | FBHIP_GRAD_DENSE.
+ * lr_device (nullable): the learning rate in device memory, read instead of lr.  clip: scale the gradients so that their global norm is
+ * at most max_norm; a norm that is not finite leaves parameters, moments and step count as they were. */
+int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, const uint8_t* host_grad_types, const float* lr_device,
+                     double lr, float grad_scale, int32_t clip, float max_norm, void* stream);
 
 #ifdef __cplusplus
 }
