@@ -579,7 +579,7 @@ def main():
             barrier()
             wall = time.perf_counter() - t0
             if world > 1:
-                t = torch.tensor([wall], device=dev, dtype=torch.float64)
+                t = torch.tensor([wall], device=dev if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)      # (gloo: host memory only)
                 mine = [torch.zeros_like(t) for _ in range(world)]
                 dist.all_gather(mine, t)
                 per_rank_walls.append([float(x.item()) for x in mine])

@@ -931,8 +931,10 @@ class FBHipAgent:
             self._gb_recv.copy_(self._gb_send.view(1, -1).expand(world, -1))
         elif dist.get_backend() == "nccl":
             dist.all_gather_into_tensor(self._gb_recv.view(-1), self._gb_send)
-        else:                                             # gloo (tests: several ranks on one GPU)
-            dist.all_gather(list(self._gb_recv.unbind(0)), self._gb_send)
+        else:                                             # gloo (tests: several ranks on one GPU): host memory only
+            parts = [torch.empty(n) for _ in range(world)]
+            dist.all_gather(parts, self._gb_send.cpu())
+            self._gb_recv.copy_(torch.stack(parts))
         # [rank][matrix][row] -> [matrix][rank * B + row]
         self._gb_panels.view(6, world, B, Lz).copy_(self._gb_recv[:, :6 * B * Lz].view(world, 6, B, Lz).permute(1, 0, 2, 3))
         self._gb_disc.view(world, B).copy_(self._gb_recv[:, 6 * B * Lz:])

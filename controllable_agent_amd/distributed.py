@@ -56,6 +56,23 @@ def rank() -> int:
     return dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
 
 
+class _Done:
+    def wait(self) -> None:
+        pass
+
+
+def all_reduce(t: torch.Tensor, async_op: bool = False):
+    """``dist.all_reduce`` (sum).  gloo gets host memory only: its collectives on device tensors can hang when several ranks share a GPU,
+    so a device tensor goes through a synchronous copy to the host and back (the sums are the same, gloo adds on the host either way)."""
+    import torch.distributed as dist
+    if t.is_cuda and dist.get_backend() == "gloo":
+        h = t.detach().cpu()
+        dist.all_reduce(h)
+        t.copy_(h)
+        return _Done() if async_op else None
+    return dist.all_reduce(t, async_op=True) if async_op else dist.all_reduce(t)
+
+
 def _reduce_fb(run_phases: tp.Callable[[int], None], fb_grads: torch.Tensor, early: tp.Optional[tp.Tuple[int, int]],
                first_mask: int, live: bool) -> None:
     """FB backward + the sum-all-reduce of the FB bucket.  With ``early = (offset, count)`` (the gradients that are final after
@@ -65,11 +82,11 @@ def _reduce_fb(run_phases: tp.Callable[[int], None], fb_grads: torch.Tensor, ear
     if not live or early is None:
         run_phases(first_mask | PHASE_FB_BWD_B)
         if live:
-            dist.all_reduce(fb_grads)
+            all_reduce(fb_grads)
         return
     off, cnt = early
     run_phases(first_mask)
-    work = dist.all_reduce(fb_grads[off:off + cnt], async_op=True)
+    work = all_reduce(fb_grads[off:off + cnt], async_op=True)
     # (the actor's own forward pass rides with the target chain when the first call carries FB_FWD_TARGET; only when it shares
     # the FB backward's launches does the second half need the bit too)
     second = PHASE_ACTOR_FWD if (first_mask & PHASE_ACTOR_FWD) and not (first_mask & PHASE_FB_FWD_TARGET) else 0
@@ -85,12 +102,12 @@ def _reduce_fb(run_phases: tp.Callable[[int], None], fb_grads: torch.Tensor, ear
             from torch.distributed.distributed_c10d import _coalescing_manager
             with _coalescing_manager(device=fb_grads.device):
                 for t in rest:
-                    dist.all_reduce(t)
+                    all_reduce(t)
             return
         except (ImportError, AttributeError, TypeError, ValueError, NotImplementedError):
             _COALESCE_OK = False
     for t in rest:
-        dist.all_reduce(t)
+        all_reduce(t)
 
 
 def dp_update(run_phases: tp.Callable[[int], None], fb_grads: torch.Tensor, actor_grads: torch.Tensor,
@@ -105,7 +122,7 @@ def dp_update(run_phases: tp.Callable[[int], None], fb_grads: torch.Tensor, acto
     world = world_size()
     if exchange is not None:
         live_ = dist.is_available() and dist.is_initialized()
-        reduce = (lambda t: dist.all_reduce(t) if t.numel() > 0 else None) if live_ else (lambda t: None)
+        reduce = (lambda t: all_reduce(t) if t.numel() > 0 else None) if live_ else (lambda t: None)
         run_phases(PHASE_SAMPLE | PHASE_FB_FWD)
         exchange()
         run_phases(PHASE_FB_BWD | PHASE_ACTOR_FWD)
@@ -119,7 +136,7 @@ def dp_update(run_phases: tp.Callable[[int], None], fb_grads: torch.Tensor, acto
         return
     # (FBHIP_FORCE_PHASE_SPLIT=1 runs this schedule on a single rank too: tests / 1-GPU rehearsal of the 8-GPU path)
     live = dist.is_available() and dist.is_initialized()
-    reduce = (lambda t: dist.all_reduce(t) if t.numel() > 0 else None) if live else (lambda t: None)   # (DiscreteFBHipAgent: no actor bucket)
+    reduce = (lambda t: all_reduce(t) if t.numel() > 0 else None) if live else (lambda t: None)   # (DiscreteFBHipAgent: no actor bucket)
     # the actor's forward rides along the FB backward
     _reduce_fb(run_phases, fb_grads, early, PHASE_SAMPLE | PHASE_FB_FWD | PHASE_FB_BWD_A | PHASE_ACTOR_FWD, live)
     run_phases(PHASE_FB_STEP | PHASE_ACTOR_GRAD)
@@ -164,7 +181,7 @@ def dp_update_many(run_phases: tp.Callable[[int], None], select_set: tp.Callable
                     run_phases(head)
                 select_set(cur)
                 run_phases(PHASE_ACTOR_GRAD)
-                work = dist.all_reduce(actor_grads, async_op=True) if (live and actor_grads.numel() > 0) else None
+                work = all_reduce(actor_grads, async_op=True) if (live and actor_grads.numel() > 0) else None
                 if work is not None:
                     work.wait()
                 run_phases(PHASE_ACTOR_STEP)
@@ -173,7 +190,7 @@ def dp_update_many(run_phases: tp.Callable[[int], None], select_set: tp.Callable
                 select_set(cur)
                 continue
             run_phases(PHASE_FB_STEP | PHASE_ACTOR_GRAD)
-            work = dist.all_reduce(actor_grads, async_op=True) if (live and actor_grads.numel() > 0) else None
+            work = all_reduce(actor_grads, async_op=True) if (live and actor_grads.numel() > 0) else None
             if t + 1 < n_steps:
                 select_set(cur ^ 1)
                 run_phases(head)                     # the next step's head, under the all-reduce
