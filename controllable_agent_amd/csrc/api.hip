@@ -1370,4 +1370,73 @@ int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, cons
     return FBHIP_OK;
 }
 
+// ---- products in 8-bit integers --------------------------------------------------------------------------------
+static int check_i8(const char* who, const void* x, const int8_t* w, int64_t ldw, const float* w_scale, const void* y, int64_t ldy, int y_type,
+                    int M, int N, int K, const void* workspace, size_t need) {
+    if (!x || !w || !w_scale || !y || M < 1 || N < 1 || K < 1) { g_err = std::string(who) + ": an operand is missing or a size is below 1"; return FBHIP_E_INVALID; }
+    if (K > FBHIP_I8_MAX_K) { g_err = std::string(who) + ": K > FBHIP_I8_MAX_K: the 32-bit sums could overflow"; return FBHIP_E_INVALID; }
+    if ((int64_t)M * (((int64_t)N + 3) / 4) > (int64_t)255 << 30) { g_err = std::string(who) + ": M * N too large"; return FBHIP_E_INVALID; }
+    if (((uintptr_t)w & 15) || (ldw & 15) || ldw < K || ldw > (int64_t)1 << 23) { g_err = std::string(who) + ": weight rows on 16-byte boundaries, K <= ldw <= 2^23 expected"; return FBHIP_E_INVALID; }
+    if (ldy < N || y_type < FBHIP_F32 || y_type > FBHIP_F16) { g_err = std::string(who) + ": ldy < N or unknown output type"; return FBHIP_E_INVALID; }
+    if (need && (!workspace || ((uintptr_t)workspace & 15))) { g_err = std::string(who) + ": workspace missing or not 16-byte aligned"; return FBHIP_E_INVALID; }
+    return FBHIP_OK;
+}
+
+static int i8_k_padded(int K) { return (K + 127) / 128 * 128; }
+
+int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* codes, int64_t ldq, float* scale, int32_t rows, int32_t K,
+                        int32_t Kp, void* stream) {
+    fbhip_ctx* none = nullptr;
+    if (!x || !codes || !scale || rows < 1 || K < 1 || Kp < K || ldx < K || ldq < Kp || x_type < FBHIP_F32 || x_type > FBHIP_F16) {
+        g_err = "fbhip_quantize_rows: bad argument"; return FBHIP_E_INVALID;
+    }
+    HIPCK(none, launch_quantize_rows(x, ldx, x_type, codes, ldq, scale, rows, K, Kp, (hipStream_t)stream));
+    return FBHIP_OK;
+}
+
+size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K) {
+    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K) return 0;
+    const I8Plan plan = gemm_i8_plan(M, N, K);
+    return plan.slices > 1 ? ((size_t)plan.slices * M * N * 4 + 15) / 16 * 16 : 0;
+}
+
+int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                  int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream) {
+    fbhip_ctx* none = nullptr;
+    RC(check_i8("fbhip_gemm_i8", a, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, fbhip_gemm_i8_workspace(M, N, K)));
+    if (!a_scale || ((uintptr_t)a & 15) || (lda & 15) || lda < K || lda > (int64_t)1 << 23) { g_err = "fbhip_gemm_i8: code rows on 16-byte boundaries, K <= lda <= 2^23, and their scales expected"; return FBHIP_E_INVALID; }
+    I8Problem p{a, w, a_scale, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, lda, ldw, ldy};
+    HIPCK(none, launch_gemm_i8(p, (int*)workspace, (hipStream_t)stream));
+    return FBHIP_OK;
+}
+
+// codes, then scales, then the product's own workspace
+static void i8_carve(int M, int K, size_t* scale_at, size_t* rest_at) {
+    *scale_at = (size_t)M * i8_k_padded(K);
+    *rest_at = *scale_at + ((size_t)M * 4 + 15) / 16 * 16;
+}
+
+size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K) {
+    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K) return 0;
+    size_t scale_at, rest_at;
+    i8_carve(M, K, &scale_at, &rest_at);
+    return rest_at + fbhip_gemm_i8_workspace(M, N, K);
+}
+
+int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                    int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream) {
+    fbhip_ctx* none = nullptr;
+    RC(check_i8("fbhip_linear_i8", x, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, 1));
+    if (ldx < K || x_type < FBHIP_F32 || x_type > FBHIP_F16) { g_err = "fbhip_linear_i8: ldx < K or unknown input type"; return FBHIP_E_INVALID; }
+    size_t scale_at, rest_at;
+    i8_carve(M, K, &scale_at, &rest_at);
+    int8_t* codes = (int8_t*)workspace;
+    float* scale = (float*)(codes + scale_at);
+    const int Kp = i8_k_padded(K);
+    HIPCK(none, launch_quantize_rows(x, ldx, x_type, codes, Kp, scale, M, K, Kp, (hipStream_t)stream));
+    I8Problem p{codes, w, scale, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, Kp, ldw, ldy};
+    HIPCK(none, launch_gemm_i8(p, (int*)(codes + rest_at), (hipStream_t)stream));
+    return FBHIP_OK;
+}
+
 }  // extern "C"

@@ -201,6 +201,20 @@ hipError_t launch_adamw_set(void* control, int64_t t, double b1, double b2, hipS
 hipError_t launch_adamw_step(const fbhip_adamw* o, const void* const* grads, const uint8_t* gtypes, const float* lr_ptr, double lr,
                              float grad_scale, int clip, float max_norm, hipStream_t s);
 
+// ---- 8-bit integer products (gemm_i8.hip)
+struct I8Problem {
+    const int8_t *a, *w;                     // [M, K] (lda) and [N, K] (ldw): rows on 16 bytes, readable to a multiple of 16
+    const float *sa, *sw, *bias;
+    void* y;
+    int* partial;                            // [slices][M][N] where K is split
+    int M, N, K, ytype, relu, yvec, steps;   // steps: of 128 along K that a workgroup takes
+    int64_t lda, ldw, ldy;
+};
+struct I8Plan { int tile, slices, steps; };
+I8Plan gemm_i8_plan(int M, int N, int K);
+hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s);
+hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s);
+
 namespace host {
 
 // ------------------------------------------------------------------------------------------------ schedule (schedule.hip)

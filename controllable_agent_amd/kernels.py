@@ -200,3 +200,121 @@ def actor_head_bwd(dt1, lnY, lnX, lnStats, lnGamma, W1a, mu, W4, P):
     check(_lib.load().fbhip_actor_head_bwd(ptr(dt1), _ld(dt1), ptr(lnY), ptr(lnX), ptr(lnStats), ptr(lnGamma), ptr(W1a), _ld(W1a), ptr(mu),
                                            _ld(mu), ptr(W4), _ld(W4), ptr(P), ptr(dpremu), La, ptr(dp), rows, H, a, stream_ptr()))
     return dpremu[:, :a], dp
+
+
+# ------------------------------------------------------------------------------------------------------ products in 8-bit integers
+_TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_checked_devices: tp.Set[int] = set()
+
+
+def _stream_on(t: torch.Tensor) -> int:
+    """The current stream of ``t``'s device, which has to be the current device; the device itself is looked at once."""
+    index = t.device.index
+    if index is None or index != torch.cuda.current_device():
+        raise ValueError(f"tensors on the current device expected, got {t.device}")
+    if index not in _checked_devices:
+        _lib.require_device()
+        _checked_devices.add(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _float_rows(x: torch.Tensor, name: str) -> tp.Tuple[int, int, int, int]:
+    """(rows, K, row stride, type) of a 2-D float matrix whose rows are contiguous"""
+    if x.dim() != 2 or x.dtype not in _TYPE_CODE or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"{name}: a float32, bfloat16 or float16 matrix with contiguous rows expected, got {x.dtype} {tuple(x.shape)} strides {x.stride()}")
+    rows, K = x.shape
+    ld = x.stride(0) if rows > 1 else max(K, 1)
+    if ld < K:
+        raise ValueError(f"{name}: rows overlap (stride {ld} for {K} columns)")
+    return rows, K, ld, _TYPE_CODE[x.dtype]
+
+
+def _code_rows(q: torch.Tensor, scale: torch.Tensor, name: str) -> tp.Tuple[int, int, int]:
+    """(rows, K, row stride) of an int8 matrix on 16-byte rows, and its scales' check"""
+    if q.dim() != 2 or q.dtype != torch.int8 or (q.shape[1] > 1 and q.stride(1) != 1):
+        raise ValueError(f"{name}: an int8 matrix with contiguous rows expected, got {q.dtype} {tuple(q.shape)} strides {q.stride()}")
+    rows, K = q.shape
+    K16 = (K + 15) // 16 * 16
+    ld = q.stride(0) if rows > 1 else K16
+    if q.numel() and (ld % 16 or ld < K or q.data_ptr() % 16 or
+                      q.untyped_storage().nbytes() - q.storage_offset() < (rows - 1) * ld + K16):
+        raise ValueError(f"{name}: rows on 16-byte boundaries that can be read to a multiple of 16 expected (quantize_rows makes them), got strides {q.stride()}")
+    if scale.dtype != torch.float32 or scale.shape != (rows,) or (rows > 1 and scale.stride(0) != 1) or scale.device != q.device:
+        raise ValueError(f"{name}: a contiguous float32 scale for each of the {rows} rows expected, got {scale.dtype} {tuple(scale.shape)}")
+    return rows, K, ld
+
+
+def _i8_output(out, out_dtype, bias, M, N, device):
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1) or bias.device != device):
+        raise ValueError(f"bias: {N} contiguous float32 on {device} expected, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    if out is None:
+        if out_dtype not in _TYPE_CODE:
+            raise ValueError(f"out_dtype: float32, bfloat16 or float16 expected, got {out_dtype}")
+        return torch.empty((M, N), dtype=out_dtype, device=device), N
+    rows, cols, ld, _ = _float_rows(out, "out")
+    if (rows, cols) != (M, N) or out.device != device:
+        raise ValueError(f"out: [{M}, {N}] on {device} expected, got {tuple(out.shape)} on {out.device}")
+    return out, ld
+
+
+def quantize_rows(x: torch.Tensor) -> tp.Tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scale): scale[r] = max|x[r]| / 127, codes = nearest whole numbers to x / scale (int8, ties to even).
+
+    The tokens of an activation matrix and the channels of a weight matrix [out, in] alike.  x: float32, bfloat16 or float16 [rows, K] with contiguous
+    rows.  ``codes`` is a view of rows padded with zeros to a multiple of 128, which ``gemm_i8`` and ``linear_i8`` read as it is.  A row that holds a NaN or an
+    infinity gets the scale NaN, so that its products are NaN; a row of zeros gets the scale 0.
+    """
+    rows, K, ld, code = _float_rows(x, "x")
+    stream = _stream_on(x)
+    Kp = (K + 127) // 128 * 128
+    q = torch.empty((rows, Kp), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows and K:
+        check(_lib.load().fbhip_quantize_rows(x.data_ptr(), ld, code, q.data_ptr(), Kp, scale.data_ptr(), rows, K, Kp, stream))
+    elif rows:
+        scale.zero_()
+    return q[:, :K], scale
+
+
+def gemm_i8(A: torch.Tensor, a_scale: torch.Tensor, B: torch.Tensor, b_scale: torch.Tensor, *, bias: tp.Optional[torch.Tensor] = None,
+            relu: bool = False, out_dtype: torch.dtype = torch.float32, out: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
+    """C[m, n] = act((sum_k A[m, k] B[n, k]) * a_scale[m] * b_scale[n] + bias[n]) on int8 codes A [M, K] (tokens) and B [N, K] (channels).
+
+    The sums are exact (K <= 131072).  Rows lie on 16-byte boundaries and can be read to a multiple of 16, as ``quantize_rows`` makes them.
+    """
+    M, K, lda = _code_rows(A, a_scale, "A")
+    N, K2, ldb = _code_rows(B, b_scale, "B")
+    if K != K2 or A.device != B.device:
+        raise ValueError(f"A {tuple(A.shape)} on {A.device} and B {tuple(B.shape)} on {B.device} do not go together")
+    stream = _stream_on(A)
+    C, ldc = _i8_output(out, out_dtype, bias, M, N, A.device)
+    if M == 0 or N == 0:
+        return C
+    lib = _lib.load()
+    need = lib.fbhip_gemm_i8_workspace(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=A.device) if need else None
+    check(lib.fbhip_gemm_i8(A.data_ptr(), lda, a_scale.data_ptr(), B.data_ptr(), ldb, b_scale.data_ptr(), ptr(bias), int(relu), C.data_ptr(), ldc,
+                            _TYPE_CODE[C.dtype], M, N, K, ptr(ws), stream))
+    return C
+
+
+def linear_i8(x: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, *, bias: tp.Optional[torch.Tensor] = None, relu: bool = False,
+              out_dtype: tp.Optional[torch.dtype] = None, out: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x W^T + bias) with x quantised row by row on the way: ``gemm_i8(*quantize_rows(x), W, w_scale, ...)`` in one call.
+
+    x: float32, bfloat16 or float16 [M, K] with contiguous rows; W, w_scale: ``quantize_rows`` of the [N, K] weights; the output has x's type
+    unless ``out_dtype`` or ``out`` says otherwise.
+    """
+    M, K, ldx, code = _float_rows(x, "x")
+    N, K2, ldw = _code_rows(W, w_scale, "W")
+    if K != K2 or x.device != W.device:
+        raise ValueError(f"x {tuple(x.shape)} on {x.device} and W {tuple(W.shape)} on {W.device} do not go together")
+    stream = _stream_on(x)
+    y, ldy = _i8_output(out, x.dtype if out_dtype is None else out_dtype, bias, M, N, x.device)
+    if M == 0 or N == 0:
+        return y
+    lib = _lib.load()
+    ws = torch.empty(lib.fbhip_linear_i8_workspace(M, N, K), dtype=torch.uint8, device=x.device)
+    check(lib.fbhip_linear_i8(x.data_ptr(), ldx, code, W.data_ptr(), ldw, w_scale.data_ptr(), ptr(bias), int(relu), y.data_ptr(), ldy,
+                              _TYPE_CODE[y.dtype], M, N, K, ws.data_ptr(), stream))
+    return y

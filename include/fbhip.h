@@ -516,6 +516,24 @@ int fbhip_adamw_set_step(const fbhip_adamw* opt, int64_t step, void* stream);
 int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, const uint8_t* host_grad_types, const float* lr_device,
                      double lr, float grad_scale, int32_t clip, float max_norm, void* stream);
 
+/* ---- matrix product in 8-bit integers (csrc/gemm_i8.hip) -------------------------------------------- */
+#define FBHIP_I8_MAX_K 131072              /* the int32 sums cannot overflow up to here */
+/* scale[r] = max|x[r, :]| / 127, codes[r, k] = nearest whole number to x[r, k] / scale[r] (ties to even).  x: FBHIP_F32 / BF16 / F16, rows
+ * ldx elements apart.  codes: rows ldq bytes apart, ldq >= Kp; columns K .. Kp - 1 are set to 0.  A row with a NaN or an infinity: scale NaN,
+ * codes 0; a row of zeros: scale 0, codes 0. */
+int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* codes, int64_t ldq, float* scale, int32_t rows, int32_t K,
+                        int32_t Kp, void* stream);
+/* y[m, n] = act((sum_k a[m, k] w[n, k]) * a_scale[m] * w_scale[n] + bias[n]).  a, w: 8-bit codes, rows on 16-byte boundaries and readable to the
+ * next multiple of 16 (what lies behind K does not count).  bias nullable; relu: 0 / 1; y: FBHIP_F32 / BF16 / F16, rows ldy elements apart.
+ * workspace: fbhip_gemm_i8_workspace bytes (16-byte aligned; nullable where that is 0). */
+size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K);
+int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                  int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);
+/* The same with x quantised row by row on the way (fbhip_quantize_rows into the workspace). */
+size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K);
+int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                    int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
