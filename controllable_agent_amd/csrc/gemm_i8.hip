@@ -132,29 +132,35 @@ __device__ __forceinline__ void i8_load_lds(uint32_t lds, uint32_t offset, const
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-// the products of one step; TAIL: only `left` codes of it belong to K (the other operand may hold anything there)
-template <class T, int WN, int FN, int FM, bool TAIL>
-__device__ __forceinline__ void i8_step(const int8_t* st, int wn, int wm, int l31, int half, int left, intx16 (&acc)[FN][FM]) {
+// the operands of one matrix instruction along K (32 codes): slice kk of a step
+template <class T, int FN, int FM>
+__device__ __forceinline__ void i8_fragments(const int8_t* st, int kk, int wn, int wm, int l31, int half, intx4 (&w)[FN], intx4 (&a)[FM]) {
+    const int piece = 2 * kk + half;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-        intx4 w[FN], a[FM];
-        const int piece = 2 * kk + half;
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-            const int row = (wn * FN + i) * 32 + l31;
-            w[i] = *(const intx4*)(st + row * I8_BK + ((piece ^ (row & 7)) * 16));
-        }
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int row = T::BN + (wm * FM + j) * 32 + l31;
-            a[j] = *(const intx4*)(st + row * I8_BK + ((piece ^ (row & 7)) * 16));
-            if (TAIL) a[j] = i8_mask(a[j], left - piece * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], a[j], acc[i][j], 0, 0, 0);
+    for (int i = 0; i < FN; ++i) {
+        const int row = (wn * FN + i) * 32 + l31;
+        w[i] = *(const intx4*)(st + row * I8_BK + ((piece ^ (row & 7)) * 16));
     }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int row = T::BN + (wm * FM + j) * 32 + l31;
+        a[j] = *(const intx4*)(st + row * I8_BK + ((piece ^ (row & 7)) * 16));
+    }
+}
+
+template <int FN, int FM>
+__device__ __forceinline__ void i8_multiply(const intx4 (&w)[FN], const intx4 (&a)[FM], intx16 (&acc)[FN][FM]) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], a[j], acc[i][j], 0, 0, 0);
+}
+
+// the first step's tile has landed; the second's loads may be under way
+template <int PIECES>
+__device__ __forceinline__ void i8_wait(bool second) {
+    if (second) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 template <int WN, int WM, int FN, int FM>
@@ -166,7 +172,9 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM>::THREADS)) gemm_i8_ker
     // workgroup b runs on XCD b % 8: each XCD takes one run of the tiles
     const int xcd = blockIdx.x & 7, each = tiles >> 3, rest = tiles & 7;
     const int t = (xcd < rest ? xcd * (each + 1) : rest * (each + 1) + (xcd - rest) * each) + ((int)blockIdx.x >> 3);
-    const int n0 = (t % tiles_n) * T::BN, m0 = (t / tiles_n) * T::BM;
+    // ... in blocks of eight token tiles, so that its 32 CUs share 8 + 4 tiles' operands and not 1 + 32
+    const int group = t / (8 * tiles_n), g0 = group * 8, gm = min(8, tiles_m - g0), in_group = t - group * 8 * tiles_n;
+    const int n0 = (in_group / gm) * T::BN, m0 = (g0 + in_group % gm) * T::BM;
     const int steps_all = (p.K + I8_BK - 1) / I8_BK;
     const int k_first = blockIdx.y * p.steps, steps = min(p.steps, steps_all - k_first);
     const bool tail = k_first + steps == steps_all && (p.K & (I8_BK - 1)) != 0;
@@ -204,15 +212,40 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM>::THREADS)) gemm_i8_ker
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
+    // The fragments of a slice are read while the slice before it is multiplied.  Before the last slice of a step everybody has read the
+    // step's tile, and the next step's has landed: the one after it goes into the same place, with a whole step's time to arrive.
+    const int full = steps - (tail ? 1 : 0);
+    intx4 w[2][FN], a[2][FM];
     issue(0);
-    for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (steps > 1) issue(1);
+    i8_wait<T::PIECES>(steps > 1);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    i8_fragments<T>(smem, 0, wn, wm, l31, half, w[0], a[0]);
+    for (int s = 0; s < full; ++s) {
+        const int8_t *st = smem + (s & 1) * T::STAGE, *next = smem + ((s + 1) & 1) * T::STAGE;
+        i8_fragments<T>(st, 1, wn, wm, l31, half, w[1], a[1]);
+        i8_multiply(w[0], a[0], acc);
+        i8_fragments<T>(st, 2, wn, wm, l31, half, w[0], a[0]);
+        i8_multiply(w[1], a[1], acc);
+        i8_fragments<T>(st, 3, wn, wm, l31, half, w[1], a[1]);
+        i8_multiply(w[0], a[0], acc);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 1 < steps) issue(s + 1);
-        const int8_t* st = smem + (s & 1) * T::STAGE;
-        if (tail && s == steps - 1) i8_step<T, WN, FN, FM, true>(st, wn, wm, l31, half, p.K - (steps_all - 1) * I8_BK, acc);
-        else i8_step<T, WN, FN, FM, false>(st, wn, wm, l31, half, 0, acc);
+        if (s + 2 < steps) issue(s + 2);
+        i8_fragments<T>(next, 0, wn, wm, l31, half, w[0], a[0]);       // (behind the last step: not used)
+        i8_multiply(w[1], a[1], acc);
+    }
+    if (tail) {          // only `left` codes of the last step belong to K; the other operand may hold anything behind them
+        const int left = p.K - (steps_all - 1) * I8_BK;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            i8_fragments<T>(smem + (full & 1) * T::STAGE, kk, wn, wm, l31, half, w[0], a[0]);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) a[0][j] = i8_mask(a[0][j], left - (2 * kk + half) * 16);
+            i8_multiply(w[0], a[0], acc);
+        }
     }
 #pragma unroll
     for (int i = 0; i < FN; ++i)
