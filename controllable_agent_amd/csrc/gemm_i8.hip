@@ -29,79 +29,187 @@ __device__ __forceinline__ float i8_load(const void* x, size_t i, int type) {
     return (float)f;
 }
 
-// One workgroup takes a row.  A row that holds a NaN or an infinity gets the scale NaN (and codes 0): its whole output row is NaN.  A row of zeros,
-// or one so small that its scale is 0, gets codes 0.
+// The code of x in a row of scale s: x / s, rounded to float32 and then to the nearest whole number, ties to even.  x times the reciprocal is off by
+// less than 5e-5 for |x / s| <= 127 (a step of v_rcp_f32, half a step of the product and of the quotient: 127 * 2.5 * 2^-23 = 3.8e-5), so that only
+// a value that comes so near to a half is divided.  Scales below 2^-100 (the reciprocal would leave the range) are divided always.
+__device__ __forceinline__ int i8_code(float x, float s, float inv) {
+    const float q = x * inv;
+    float r = rintf(q);
+    if (!(fabsf(q - r) < 0.49995f)) r = fminf(fmaxf(rintf(x / s), -127.f), 127.f);
+    return (int)r;
+}
+
+struct I8Row { float scale, inv; bool zero; };
+// a row that holds a NaN or an infinity: the scale NaN and codes 0; a row of zeros, or one so small that its scale is 0: codes 0
+__device__ __forceinline__ I8Row i8_row(float top, bool bad) {
+    I8Row r;
+    r.scale = top / 127.f;
+    r.zero = bad || r.scale == 0.f;
+    r.inv = r.scale >= 0x1p-100f ? __builtin_amdgcn_rcpf(r.scale) : __uint_as_float(0x7FC00000u);
+    if (bad) r.scale = __uint_as_float(0x7FC00000u);
+    return r;
+}
+
+__device__ __forceinline__ bool i8_no_number(float x) { return !(fabsf(x) < __uint_as_float(0x7F800000u)); }
+
+// A row in the registers of TPR threads: C pieces of 16 bytes a thread, read once.  Rows on 16-byte boundaries, K in whole pieces or not.
+// (One thread row of 64 takes up to 8 pieces: 2048 fp32 or 4096 16-bit values; a workgroup of 256 four times that.)
+template <int TPR, int C, bool WIDE>
+__global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
+                                                                float* __restrict__ scale, int rows, int K, int Kp) {
+    constexpr int V = WIDE ? 4 : 8;                       // values of a piece (WIDE: fp32)
+    __shared__ float red[4];
+    __shared__ int reds[4];
+    const int t = threadIdx.x % TPR, row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const bool live = row < rows;                         // (only TPR = 64 has rows behind the end)
+    const char* base = (const char*)x + (size_t)(live ? row : rows - 1) * ldx * (16 / V);
+    float v[C][V];
+    float top = 0.f;
+    bool odd = false;
+    uint4 raw[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k = (c * TPR + t) * V;
+        raw[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (k + V <= K) raw[c] = *(const uint4*)(base + (size_t)k * (16 / V));
+        else if (k < K) {                                 // the piece that the row ends in
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            for (int e = 0; e < K - k; ++e) {
+                if (WIDE) w[e] = ((const uint32_t*)base)[k + e];
+                else w[e >> 1] |= (uint32_t)((const uint16_t*)base)[k + e] << (16 * (e & 1));
+            }
+            raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float f;
+            if (WIDE) f = __uint_as_float(w[e & 3]);
+            else if (type == FBHIP_BF16) f = __uint_as_float((e & 1) ? w[(e >> 1) & 3] & 0xFFFF0000u : w[(e >> 1) & 3] << 16);
+            else {
+                const uint16_t h = (uint16_t)(w[(e >> 1) & 3] >> (16 * (e & 1)));
+                _Float16 g;
+                __builtin_memcpy(&g, &h, 2);
+                f = (float)g;
+            }
+            v[c][e] = f;
+            odd = odd || i8_no_number(f);
+            top = fmaxf(top, fabsf(f));
+        }
+    }
+    top = wave_max(top);
+    int bad = __any(odd);
+    if (TPR == 256) {
+        if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = top; reds[threadIdx.x >> 6] = bad; }
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        bad = reds[0] | reds[1] | reds[2] | reds[3];
+    }
+    const I8Row r = i8_row(top, bad != 0);
+    if (!live) return;
+    int8_t* out = q + (size_t)row * ldq;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k = (c * TPR + t) * V;
+        if (k >= Kp) break;
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int code = r.zero ? 0 : i8_code(v[c][e], r.scale, r.inv);      // (zeros behind K stay zeros)
+            w[e >> 2] |= (uint32_t)(code & 0xFF) << (8 * (e & 3));
+        }
+        if (WIDE) *(uint32_t*)(out + k) = w[0];
+        else *(uint2*)(out + k) = make_uint2(w[0], w[1]);
+    }
+    if (t == 0) scale[row] = r.scale;
+}
+
+// Any row: a workgroup reads it twice.
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
                                                             float* __restrict__ scale, int K, int Kp) {
     __shared__ float red[4];
-    __shared__ int bad;
+    __shared__ int reds[4];
     const int tid = threadIdx.x;
     const size_t base = (size_t)blockIdx.x * ldx;
-    if (tid == 0) bad = 0;
-    __syncthreads();
     float top = 0.f;
     bool odd = false;
     for (int k = tid; k < K; k += 256) {
-        const float v = fabsf(i8_load(x, base + k, type));
-        odd = odd || !(v < __uint_as_float(0x7F800000u));
-        top = fmaxf(top, v);
+        const float v = i8_load(x, base + k, type);
+        odd = odd || i8_no_number(v);
+        top = fmaxf(top, fabsf(v));
     }
     top = wave_max(top);
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    if (odd) bad = 1;
+    const int bad = __any(odd);
+    if ((tid & 63) == 0) { red[tid >> 6] = top; reds[tid >> 6] = bad; }
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float s = top / 127.f;
-    const bool zero = bad || s == 0.f;
-    for (int k = tid; k < Kp; k += 256) {
-        float c = 0.f;
-        if (k < K && !zero) c = fminf(fmaxf(rintf(i8_load(x, base + k, type) / s), -127.f), 127.f);
-        q[(size_t)blockIdx.x * ldq + k] = (int8_t)(int)c;
-    }
-    if (tid == 0) scale[blockIdx.x] = bad ? __uint_as_float(0x7FC00000u) : s;
+    const I8Row r = i8_row(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), (reds[0] | reds[1] | reds[2] | reds[3]) != 0);
+    for (int k = tid; k < Kp; k += 256)
+        q[(size_t)blockIdx.x * ldq + k] = (int8_t)(k < K && !r.zero ? i8_code(i8_load(x, base + k, type), r.scale, r.inv) : 0);
+    if (tid == 0) scale[blockIdx.x] = r.scale;
+}
+
+template <int TPR, int C>
+static void launch_quantize_reg(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s) {
+    const dim3 grid((rows + 256 / TPR - 1) / (256 / TPR));
+    if (type == FBHIP_F32) hipLaunchKernelGGL((quantize_rows_reg_kernel<TPR, C, true>), grid, dim3(256), 0, s, x, ldx, type, q, ldq, scale, rows, K, Kp);
+    else hipLaunchKernelGGL((quantize_rows_reg_kernel<TPR, C, false>), grid, dim3(256), 0, s, x, ldx, type, q, ldq, scale, rows, K, Kp);
 }
 
 hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s) {
-    hipLaunchKernelGGL(quantize_rows_kernel, dim3(rows), dim3(256), 0, s, x, ldx, type, q, ldq, scale, K, Kp);
+    const int V = type == FBHIP_F32 ? 4 : 8, size = 16 / V;
+    const bool aligned = ((uintptr_t)x & 15) == 0 && (ldx * size) % 16 == 0 && ((uintptr_t)q & 7) == 0 && ldq % 8 == 0 && Kp % 8 == 0;
+    const int pieces = (Kp + V - 1) / V;
+    // a wave for a row while a row fits, unless the rows are so few that more threads a row fill the CUs sooner
+    if (aligned && pieces <= 64 * 2) launch_quantize_reg<64, 2>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (aligned && pieces <= 64 * 4 && rows >= 2048) launch_quantize_reg<64, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (aligned && pieces <= 256) launch_quantize_reg<256, 1>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (aligned && pieces <= 256 * 4) launch_quantize_reg<256, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (aligned && pieces <= 256 * 8) launch_quantize_reg<256, 8>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else hipLaunchKernelGGL(quantize_rows_kernel, dim3(rows), dim3(256), 0, s, x, ldx, type, q, ldq, scale, K, Kp);
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------------------------------------------------------------ epilogue
-// y[m, n .. n+3] from the sums of four neighbouring columns
-__device__ __forceinline__ void i8_store4(const I8Problem& p, int m, int n, int a0, int a1, int a2, int a3) {
-    if (m >= p.M || n >= p.N) return;
-    const float sa = p.sa[m];
-    const int acc[4] = {a0, a1, a2, a3};
-    float y[4];
+// y[m, n .. n+3] from the sums of four neighbouring columns; the scales and the bias are the caller's
+__device__ __forceinline__ void i8_store4(const I8Problem& p, int m, int n, const int (&acc)[4], float sa, float4 sw, float4 bias) {
+    float y[4] = {(float)acc[0] * sa * sw.x + bias.x, (float)acc[1] * sa * sw.y + bias.y, (float)acc[2] * sa * sw.z + bias.z,
+                  (float)acc[3] * sa * sw.w + bias.w};
+    if (p.relu) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int c = min(n + j, p.N - 1);
-        y[j] = (float)acc[j] * sa * p.sw[c];
-        if (p.bias != nullptr) y[j] += p.bias[c];
-        if (p.relu) y[j] = y[j] < 0.f ? 0.f : y[j];          // (NaN stays)
+        for (int j = 0; j < 4; ++j) y[j] = y[j] < 0.f ? 0.f : y[j];          // (NaN stays)
     }
     const size_t at = (size_t)m * p.ldy + n;
+    const bool whole = p.yvec && n + 3 < p.N;
     if (p.ytype == FBHIP_F32) {
         float* o = (float*)p.y + at;
-        if (p.yvec && n + 3 < p.N) { *(float4*)o = make_float4(y[0], y[1], y[2], y[3]); return; }
-        for (int j = 0; j < 4 && n + j < p.N; ++j) o[j] = y[j];
+        if (whole) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
+        else
+            for (int j = 0; j < 4; ++j) if (n + j < p.N) o[j] = y[j];
         return;
     }
-    uint16_t h[4];
+    uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (p.ytype == FBHIP_BF16) {
             const uint32_t b = __float_as_uint(y[j]);
-            h[j] = y[j] != y[j] ? 0x7FC0 : (uint16_t)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);       // nearest, ties to even
+            h[j] = y[j] != y[j] ? 0x7FC0u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;       // nearest, ties to even
         } else {
             const _Float16 f = (_Float16)y[j];
-            __builtin_memcpy(&h[j], &f, 2);
+            uint16_t u;
+            __builtin_memcpy(&u, &f, 2);
+            h[j] = u;
         }
     }
     uint16_t* o = (uint16_t*)p.y + at;
-    if (p.yvec && n + 3 < p.N) { *(uint2*)o = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16); return; }
-    for (int j = 0; j < 4 && n + j < p.N; ++j) o[j] = h[j];
+    if (whole) *(uint2*)o = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    else
+        for (int j = 0; j < 4; ++j) if (n + j < p.N) o[j] = (uint16_t)h[j];
 }
+
+__device__ __forceinline__ float i8_channel(const float* v, int n, int N) { return v != nullptr ? v[min(n, N - 1)] : 0.f; }
 
 // the last `valid` (1..15, or more: all) of a lane's 16 codes of the K dimension stay
 __device__ __forceinline__ intx4 i8_mask(intx4 v, int valid) {
@@ -116,14 +224,17 @@ __device__ __forceinline__ intx4 i8_mask(intx4 v, int valid) {
 // ------------------------------------------------------------------------------------------------------------------ tiles
 // A workgroup of WN x WM waves computes a tile of (WN FN 32) channels x (WM FM 32) tokens; a wave keeps FN x FM accumulators of the
 // 32x32x32 matrix instruction, the weights as its first operand, so that a lane holds four neighbouring channels of one token.
-// Both operands come in rows of 128 bytes straight into shared memory (16 bytes a lane), two steps ahead.  The 16-byte pieces of row r are
-// stored in the order piece ^ (r & 7): eight rows' pieces of the same place fall into different banks.
-template <int WN, int WM, int FN, int FM>
+// A step takes BK bytes of K: both operands' rows of it come straight into shared memory (16 bytes a lane), S steps deep.  Shared memory
+// has 64 banks: a fragment read of 16 rows' 16-byte pieces is free of conflicts if rows that lie a multiple of 256 bytes apart keep them in
+// different places, so the pieces of row r are stored in the order piece ^ (r / (256 / BK)).
+template <int WN, int WM, int FN, int FM, int BK_, int S_>
 struct I8Tile {
-    static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES, BN = WN * FN * 32, BM = WM * FM * 32, ROWS = BN + BM;
-    static constexpr int PIECES = ROWS / 8 / WAVES;            // 1 KB loads a wave issues for a step
-    static constexpr int STAGE = ROWS * I8_BK, LDS = 2 * STAGE;
-    static_assert(ROWS % (8 * WAVES) == 0 && LDS <= 160 * 1024, "tile");
+    static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES, BN = WN * FN * 32, BM = WM * FM * 32, ROWS = BN + BM, BK = BK_, S = S_;
+    static constexpr int PER_ROW = BK / 16, PIECE_ROWS = 64 / PER_ROW;      // 16-byte pieces of a row; rows of a 1 KB load
+    static constexpr int PIECES = ROWS / PIECE_ROWS / WAVES;                // loads a wave issues for a step
+    static constexpr int SLICES = BK / 32, STAGE = ROWS * BK, LDS = S * STAGE + (2 * BN + BM) * 4;
+    static_assert(ROWS % (PIECE_ROWS * WAVES) == 0 && LDS <= 160 * 1024 && (BK == 64 || BK == 128), "tile");
+    static __device__ __forceinline__ int place(int row, int piece) { return (piece ^ ((row / (256 / BK)) & (PER_ROW - 1))) * 16; }
 };
 
 // 1 KB of global memory into shared memory, lane l's 16 bytes behind lane l-1's.  (Assembly: the compiler would wait for all such
@@ -132,40 +243,23 @@ __device__ __forceinline__ void i8_load_lds(uint32_t lds, uint32_t offset, const
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-// the operands of one matrix instruction along K (32 codes): slice kk of a step
+template <int COUNT>
+__device__ __forceinline__ void i8_wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory"); }
+
+// The operands of one matrix instruction along K (32 codes), slice kk of a step: `w0` / `a0` is where the lane's first row keeps its piece of
+// slice 0; the rows of the other fragments lie 32 rows on, and slice kk's piece is 2 kk pieces away, by exclusive or.
 template <class T, int FN, int FM>
-__device__ __forceinline__ void i8_fragments(const int8_t* st, int kk, int wn, int wm, int l31, int half, intx4 (&w)[FN], intx4 (&a)[FM]) {
-    const int piece = 2 * kk + half;
+__device__ __forceinline__ void i8_fragments(const int8_t* st, int kk, uint32_t w0, uint32_t a0, intx4 (&w)[FN], intx4 (&a)[FM]) {
+    const int8_t *wp = st + (w0 ^ (kk * 32)), *ap = st + (a0 ^ (kk * 32));
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-        const int row = (wn * FN + i) * 32 + l31;
-        w[i] = *(const intx4*)(st + row * I8_BK + ((piece ^ (row & 7)) * 16));
-    }
+    for (int i = 0; i < FN; ++i) w[i] = *(const intx4*)(wp + i * 32 * T::BK);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const int row = T::BN + (wm * FM + j) * 32 + l31;
-        a[j] = *(const intx4*)(st + row * I8_BK + ((piece ^ (row & 7)) * 16));
-    }
+    for (int j = 0; j < FM; ++j) a[j] = *(const intx4*)(ap + j * 32 * T::BK);
 }
 
-template <int FN, int FM>
-__device__ __forceinline__ void i8_multiply(const intx4 (&w)[FN], const intx4 (&a)[FM], intx16 (&acc)[FN][FM]) {
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], a[j], acc[i][j], 0, 0, 0);
-}
-
-// the first step's tile has landed; the second's loads may be under way
-template <int PIECES>
-__device__ __forceinline__ void i8_wait(bool second) {
-    if (second) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-}
-
-template <int WN, int WM, int FN, int FM>
-__global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM>::THREADS)) gemm_i8_kernel(const I8Problem p) {
-    using T = I8Tile<WN, WM, FN, FM>;
+template <int WN, int WM, int FN, int FM, int BK, int S>
+__global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN * FM <= 4 ? 4 : 2)) gemm_i8_kernel(const I8Problem p) {
+    using T = I8Tile<WN, WM, FN, FM, BK, S>;
     extern __shared__ __attribute__((aligned(1024))) int8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_n = (p.N + T::BN - 1) / T::BN, tiles_m = (p.M + T::BM - 1) / T::BM, tiles = tiles_n * tiles_m;
@@ -175,35 +269,41 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM>::THREADS)) gemm_i8_ker
     // ... in blocks of eight token tiles, so that its 32 CUs share 8 + 4 tiles' operands and not 1 + 32
     const int group = t / (8 * tiles_n), g0 = group * 8, gm = min(8, tiles_m - g0), in_group = t - group * 8 * tiles_n;
     const int n0 = (in_group / gm) * T::BN, m0 = (g0 + in_group % gm) * T::BM;
-    const int steps_all = (p.K + I8_BK - 1) / I8_BK;
+    const int steps_all = (p.K + BK - 1) / BK;
     const int k_first = blockIdx.y * p.steps, steps = min(p.steps, steps_all - k_first);
-    const bool tail = k_first + steps == steps_all && (p.K & (I8_BK - 1)) != 0;
+    const bool tail = k_first + steps == steps_all && (p.K & (BK - 1)) != 0;
 
-    // where this lane loads from: row (lane >> 3) of each 8-row piece, 16-byte piece (lane & 7) ^ row
-    const int r8 = lane >> 3, c16 = ((lane & 7) ^ r8) * 16;
+    // where this lane loads from: row lane / PER_ROW of each 1 KB of rows
     uint32_t off[T::PIECES];
 #pragma unroll
     for (int q = 0; q < T::PIECES; ++q) {
-        const int row = (wave * T::PIECES + q) * 8 + r8;
+        const int row = (wave * T::PIECES + q) * T::PIECE_ROWS + lane / T::PER_ROW, c16 = T::place(row, lane % T::PER_ROW);
         off[q] = row < T::BN ? (uint32_t)min(row, p.N - 1 - n0) * (uint32_t)p.ldw + c16 : (uint32_t)min(row - T::BN, p.M - 1 - m0) * (uint32_t)p.lda + c16;
     }
-    // the last step of an uneven K reads no further than the 16 bytes that hold the row's end
-    const int k16 = (p.K + 15) & ~15;
-    const uint32_t back = (uint32_t)max(0, (steps_all - 1) * I8_BK + c16 - (k16 - 16));
     const int8_t* wbase = p.w + (size_t)n0 * p.ldw;
     const int8_t* abase = p.a + (size_t)m0 * p.lda;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)smem;
-    auto issue = [&](int s) __attribute__((always_inline)) {
-        const uint32_t minus = tail && s == steps - 1 ? back : 0u;
-        const size_t k = (size_t)(k_first + s) * I8_BK;
-#pragma unroll
-        for (int q = 0; q < T::PIECES; ++q) {
-            const int piece = wave * T::PIECES + q;
-            i8_load_lds(lds0 + (uint32_t)((s & 1) * T::STAGE + piece * 1024), off[q] - minus, (piece * 8 < T::BN ? wbase : abase) + k);
+    // the last step of an uneven K reads no further than the 16 bytes that hold the row's end
+    const int k16 = (p.K + 15) & ~15, last_piece = k16 - 16 - (steps_all - 1) * BK;
+    auto issue = [&](int s, int q) __attribute__((always_inline)) {
+        const int piece = wave * T::PIECES + q;
+        uint32_t from = off[q];
+        if (tail && s == steps - 1) {
+            const int row = piece * T::PIECE_ROWS + lane / T::PER_ROW;
+            from -= (uint32_t)max(0, T::place(row, lane % T::PER_ROW) - last_piece);
         }
+        i8_load_lds(lds0 + (uint32_t)((s % S) * T::STAGE + piece * 1024), from, (piece * T::PIECE_ROWS < T::BN ? wbase : abase) + (size_t)(k_first + s) * BK);
     };
 
+    // the tile's scales and bias wait behind the tiles: at the end a lane needs 4 FN channels' and FM tokens'
+    float *sw = (float*)(smem + S * T::STAGE), *bias = sw + T::BN, *sa = bias + T::BN;
+    for (int c = threadIdx.x; c < T::BN; c += T::THREADS) { sw[c] = i8_channel(p.sw, n0 + c, p.N); bias[c] = i8_channel(p.bias, n0 + c, p.N); }
+    for (int c = threadIdx.x; c < T::BM; c += T::THREADS) sa[c] = i8_channel(p.sa, m0 + c, p.M);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");          // (the loop counts the loads that are under way)
+
     const int l31 = lane & 31, half = lane >> 5, wn = wave % WN, wm = wave / WN;
+    const int wrow = wn * FN * 32 + l31, arow = T::BN + wm * FM * 32 + l31;
+    const uint32_t w0 = wrow * BK + T::place(wrow, half), a0 = arow * BK + T::place(arow, half);
     intx16 acc[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -213,57 +313,96 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM>::THREADS)) gemm_i8_ker
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
     // The fragments of a slice are read while the slice before it is multiplied.  Before the last slice of a step everybody has read the
-    // step's tile, and the next step's has landed: the one after it goes into the same place, with a whole step's time to arrive.
+    // step's tile, and the next step's has landed: step s + S goes into the place of step s, its loads spread over a step's slices (together they
+    // would fill the CU's load queue and hold up the products behind them).
     const int full = steps - (tail ? 1 : 0);
     intx4 w[2][FN], a[2][FM];
-    issue(0);
-    if (steps > 1) issue(1);
-    i8_wait<T::PIECES>(steps > 1);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (s < steps) {
+#pragma unroll
+            for (int q = 0; q < T::PIECES; ++q) issue(s, q);
+        }
+    if (steps >= S) i8_wait_loads<(S - 1) * T::PIECES>();
+    else i8_wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    i8_fragments<T>(smem, 0, wn, wm, l31, half, w[0], a[0]);
-    for (int s = 0; s < full; ++s) {
-        const int8_t *st = smem + (s & 1) * T::STAGE, *next = smem + ((s + 1) & 1) * T::STAGE;
-        i8_fragments<T>(st, 1, wn, wm, l31, half, w[1], a[1]);
-        i8_multiply(w[0], a[0], acc);
-        i8_fragments<T>(st, 2, wn, wm, l31, half, w[0], a[0]);
-        i8_multiply(w[1], a[1], acc);
-        i8_fragments<T>(st, 3, wn, wm, l31, half, w[1], a[1]);
-        i8_multiply(w[0], a[0], acc);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + 2 < steps) issue(s + 2);
-        i8_fragments<T>(next, 0, wn, wm, l31, half, w[0], a[0]);       // (behind the last step: not used)
-        i8_multiply(w[1], a[1], acc);
-    }
-    if (tail) {          // only `left` codes of the last step belong to K; the other operand may hold anything behind them
-        const int left = p.K - (steps_all - 1) * I8_BK;
+    i8_fragments<T>(smem, 0, w0, a0, w[0], a[0]);
+    // slice `set`'s products, with share r of the loads of step `to` between them
+    auto multiply = [&](int set, int r, int to) __attribute__((always_inline)) {
+        const bool live = to >= S && to < steps;
+        const int first = r * T::PIECES / T::SLICES, count = (r + 1) * T::PIECES / T::SLICES - first;
+        int done = 0;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            i8_fragments<T>(smem + (full & 1) * T::STAGE, kk, wn, wm, l31, half, w[0], a[0]);
+        for (int i = 0; i < FN; ++i)
 #pragma unroll
-            for (int j = 0; j < FM; ++j) a[0][j] = i8_mask(a[0][j], left - (2 * kk + half) * 16);
-            i8_multiply(w[0], a[0], acc);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int m = m0 + (wm * FM + j) * 32 + l31;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int n = n0 + (wn * FN + i) * 32 + 8 * g + 4 * half;
-                const intx16& c = acc[i][j];
-                if (p.partial == nullptr) i8_store4(p, m, n, c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]);
-                else if (m < p.M) {
-                    int* o = p.partial + ((size_t)blockIdx.y * p.M + m) * p.N + n;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = c[4 * g + e];
+            for (int j = 0; j < FM; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[set][i], a[set][j], acc[i][j], 0, 0, 0);
+                if (done * FN * FM < (i * FM + j + 1) * count) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (live) issue(to, first + done);
+                    ++done;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+    };
+    for (int s = 0; s < full; ++s) {
+        const int8_t *st = smem + (s % S) * T::STAGE, *next = smem + ((s + 1) % S) * T::STAGE;
+#pragma unroll
+        for (int kk = 0; kk + 1 < T::SLICES; ++kk) {
+            i8_fragments<T>(st, kk + 1, w0, a0, w[(kk + 1) & 1], a[(kk + 1) & 1]);
+            multiply(kk & 1, kk + 1, s - 1 + S);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (s + S <= steps) i8_wait_loads<(S - 2) * T::PIECES>();
+        else i8_wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        i8_fragments<T>(next, 0, w0, a0, w[0], a[0]);       // (behind the last step: not used)
+        multiply((T::SLICES - 1) & 1, 0, s + S);
+    }
+    if (tail) {          // only `left` codes of the last step belong to K; the other operand may hold anything behind them
+        const int left = p.K - (steps_all - 1) * BK;
+#pragma unroll
+        for (int kk = 0; kk < T::SLICES; ++kk) {
+            i8_fragments<T>(smem + (full % S) * T::STAGE, kk, w0, a0, w[0], a[0]);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) a[0][j] = i8_mask(a[0][j], left - (2 * kk + half) * 16);
+            multiply(0, 0, 0);
+        }
+    }
+    if (p.partial != nullptr) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const int m = m0 + (wm * FM + j) * 32 + l31;
+                if (m >= p.M) continue;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int n = n0 + (wn * FN + i) * 32 + 8 * g + 4 * half;
+                    int* o = p.partial + ((size_t)blockIdx.y * p.M + m) * p.N + n;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = acc[i][j][4 * g + e];
+                }
+            }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int mt = (wm * FM + j) * 32 + l31, m = m0 + mt;
+        const float s = sa[mt];
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int nt = (wn * FN + i) * 32 + 8 * g + 4 * half;
+                if (n0 + nt >= p.N) continue;
+                const int c[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                i8_store4(p, m, n0 + nt, c, s, *(const float4*)(sw + nt), *(const float4*)(bias + nt));
+            }
+    }
 }
 
 // the sums of a K that was split over several workgroups
@@ -272,24 +411,28 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)p.M * quads) return;
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    const float sa = p.sa[m];
+    const float4 sw = make_float4(i8_channel(p.sw, n, p.N), i8_channel(p.sw, n + 1, p.N), i8_channel(p.sw, n + 2, p.N), i8_channel(p.sw, n + 3, p.N));
+    const float4 bias = make_float4(i8_channel(p.bias, n, p.N), i8_channel(p.bias, n + 1, p.N), i8_channel(p.bias, n + 2, p.N), i8_channel(p.bias, n + 3, p.N));
     int acc[4] = {0, 0, 0, 0};
     for (int s = 0; s < slices; ++s) {
         const int* o = p.partial + ((size_t)s * p.M + m) * p.N + n;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (n + e < p.N) acc[e] += o[e];
+        for (int e = 0; e < 4; ++e) acc[e] += n + e < p.N ? o[e] : 0;
     }
-    i8_store4(p, m, n, acc[0], acc[1], acc[2], acc[3]);
+    i8_store4(p, m, n, acc, sa, sw, bias);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ choice
-template <int WN, int WM, int FN, int FM>
-static hipError_t launch_i8_tile(const I8Problem& p, int slices, hipStream_t s) {
-    using T = I8Tile<WN, WM, FN, FM>;
+template <int WN, int WM, int FN, int FM, int BK, int S>
+static hipError_t launch_i8_tile(I8Problem p, int slices, hipStream_t s) {
+    using T = I8Tile<WN, WM, FN, FM, BK, S>;
     static const hipError_t prepared =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_kernel<WN, WM, FN, FM>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_kernel<WN, WM, FN, FM, BK, S>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
     if (prepared != hipSuccess) return prepared;
     const int tiles = ((p.N + T::BN - 1) / T::BN) * ((p.M + T::BM - 1) / T::BM);
-    hipLaunchKernelGGL((gemm_i8_kernel<WN, WM, FN, FM>), dim3(tiles, slices), dim3(T::THREADS), T::LDS, s, p);
+    p.steps *= I8_BK / BK;
+    hipLaunchKernelGGL((gemm_i8_kernel<WN, WM, FN, FM, BK, S>), dim3(tiles, slices), dim3(T::THREADS), T::LDS, s, p);
     return hipGetLastError();
 }
 
@@ -319,9 +462,9 @@ hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
     const size_t size = p.ytype == FBHIP_F32 ? 4 : 2;
     p.yvec = ((uintptr_t)p.y % (4 * size) == 0) && p.ldy % 4 == 0;
     hipError_t e;
-    if (plan.tile == 256) e = launch_i8_tile<2, 4, 4, 2>(p, plan.slices, s);
-    else if (plan.tile == 128) e = launch_i8_tile<2, 2, 2, 2>(p, plan.slices, s);
-    else e = launch_i8_tile<2, 2, 1, 1>(p, plan.slices, s);
+    if (plan.tile == 256) e = launch_i8_tile<4, 4, 2, 2, 128, 2>(p, plan.slices, s);
+    else if (plan.tile == 128) e = launch_i8_tile<2, 4, 2, 1, 128, 2>(p, plan.slices, s);
+    else e = launch_i8_tile<2, 2, 1, 1, 128, 2>(p, plan.slices, s);
     if (e != hipSuccess || plan.slices == 1) return e;
     const int64_t quads = (int64_t)p.M * ((p.N + 3) / 4);
     hipLaunchKernelGGL(gemm_i8_fold_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, p, plan.slices);
