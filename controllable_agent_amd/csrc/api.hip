@@ -1397,7 +1397,7 @@ int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* code
 size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K) {
     if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K) return 0;
     const I8Plan plan = gemm_i8_plan(M, N, K);
-    return plan.slices > 1 ? ((size_t)plan.slices * M * N * 4 + 15) / 16 * 16 : 0;
+    return plan.slices > 1 ? (size_t)plan.slices * M * (((size_t)N + 3) / 4) * 16 : 0;
 }
 
 int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,

@@ -173,43 +173,78 @@ hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q,
 }
 
 // ------------------------------------------------------------------------------------------------------------------ epilogue
-// y[m, n .. n+3] from the sums of four neighbouring columns; the scales and the bias are the caller's
-__device__ __forceinline__ void i8_store4(const I8Problem& p, int m, int n, const int (&acc)[4], float sa, float4 sw, float4 bias) {
-    float y[4] = {(float)acc[0] * sa * sw.x + bias.x, (float)acc[1] * sa * sw.y + bias.y, (float)acc[2] * sa * sw.z + bias.z,
-                  (float)acc[3] * sa * sw.w + bias.w};
-    if (p.relu) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = y[j] < 0.f ? 0.f : y[j];          // (NaN stays)
+__device__ __forceinline__ float i8_value(const I8Problem& p, int acc, float sa, float sw, float bias) {
+    const float y = (float)acc * sa * sw + bias;
+    return p.relu && y < 0.f ? 0.f : y;          // (NaN stays)
+}
+
+__device__ __forceinline__ uint32_t i8_half(float y, int type) {
+    if (type == FBHIP_BF16) {
+        const uint32_t b = __float_as_uint(y);
+        return y != y ? 0x7FC0u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;       // nearest, ties to even
     }
-    const size_t at = (size_t)m * p.ldy + n;
-    const bool whole = p.yvec && n + 3 < p.N;
+    const _Float16 f = (_Float16)y;
+    uint16_t u;
+    __builtin_memcpy(&u, &f, 2);
+    return u;
+}
+
+__device__ __forceinline__ float i8_channel(const float* v, int n, int N) { return v != nullptr ? v[min(n, N - 1)] : 0.f; }
+
+// up to four neighbouring values of a row
+__device__ __forceinline__ void i8_store4(const I8Problem& p, size_t at, int count, const float (&y)[4]) {
     if (p.ytype == FBHIP_F32) {
         float* o = (float*)p.y + at;
-        if (whole) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
+        if (p.yvec && count == 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
         else
-            for (int j = 0; j < 4; ++j) if (n + j < p.N) o[j] = y[j];
+            for (int j = 0; j < count; ++j) o[j] = y[j];
         return;
     }
     uint32_t h[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (p.ytype == FBHIP_BF16) {
-            const uint32_t b = __float_as_uint(y[j]);
-            h[j] = y[j] != y[j] ? 0x7FC0u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;       // nearest, ties to even
-        } else {
-            const _Float16 f = (_Float16)y[j];
-            uint16_t u;
-            __builtin_memcpy(&u, &f, 2);
-            h[j] = u;
-        }
-    }
+    for (int j = 0; j < 4; ++j) h[j] = i8_half(y[j], p.ytype);
     uint16_t* o = (uint16_t*)p.y + at;
-    if (whole) *(uint2*)o = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    if (p.yvec && count == 4) *(uint2*)o = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     else
-        for (int j = 0; j < 4; ++j) if (n + j < p.N) o[j] = (uint16_t)h[j];
+        for (int j = 0; j < count; ++j) o[j] = (uint16_t)h[j];
 }
 
-__device__ __forceinline__ float i8_channel(const float* v, int n, int N) { return v != nullptr ? v[min(n, N - 1)] : 0.f; }
+// `rows` tokens from m on, `cols` channels from n on (at most 32 x COLS), their sums in shared memory; the scales and the bias in shared memory too
+template <int COLS>
+__device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int ld, int m, int n, int rows, int cols, const float* sa, const float* sw,
+                                        const float* bias, int lane) {
+    if (p.partial != nullptr) {          // a slice of K: the sums themselves, rows padded to four
+        const int ldp = (p.N + 3) & ~3;
+        constexpr int LANES = COLS / 4;
+        int* o = p.partial + ((size_t)blockIdx.y * p.M + m) * ldp + n;
+        const int c = lane % LANES * 4;
+        if (c < cols)
+            for (int r = lane / LANES; r < rows; r += 64 / LANES) *(intx4*)(o + (size_t)r * ldp + c) = *(const intx4*)(box + r * ld + c);
+        return;
+    }
+    if (p.yvec) {
+        constexpr int LANES = COLS / 4;
+        const int c = lane % LANES * 4;
+        if (c >= cols) return;
+        const float4 s = *(const float4*)(sw + c), b = *(const float4*)(bias + c);
+        for (int r = lane / LANES; r < rows; r += 64 / LANES) {
+            const intx4 v = *(const intx4*)(box + r * ld + c);
+            const float t = sa[r];
+            const float y[4] = {i8_value(p, v[0], t, s.x, b.x), i8_value(p, v[1], t, s.y, b.y), i8_value(p, v[2], t, s.z, b.z), i8_value(p, v[3], t, s.w, b.w)};
+            i8_store4(p, (size_t)(m + r) * p.ldy + n + c, min(4, cols - c), y);
+        }
+        return;
+    }
+    const int c = lane % COLS;           // one value a lane
+    if (c >= cols) return;
+    const float s = sw[c], b = bias[c];
+    for (int r = lane / COLS; r < rows; r += 64 / COLS) {
+        const float y = i8_value(p, box[r * ld + c], sa[r], s, b);
+        const size_t at = (size_t)(m + r) * p.ldy + n + c;
+        if (p.ytype == FBHIP_F32) ((float*)p.y)[at] = y;
+        else ((uint16_t*)p.y)[at] = (uint16_t)i8_half(y, p.ytype);
+    }
+}
 
 // the last `valid` (1..15, or more: all) of a lane's 16 codes of the K dimension stay
 __device__ __forceinline__ intx4 i8_mask(intx4 v, int valid) {
@@ -232,7 +267,9 @@ struct I8Tile {
     static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES, BN = WN * FN * 32, BM = WM * FM * 32, ROWS = BN + BM, BK = BK_, S = S_;
     static constexpr int PER_ROW = BK / 16, PIECE_ROWS = 64 / PER_ROW;      // 16-byte pieces of a row; rows of a 1 KB load
     static constexpr int PIECES = ROWS / PIECE_ROWS / WAVES;                // loads a wave issues for a step
-    static constexpr int SLICES = BK / 32, STAGE = ROWS * BK, LDS = S * STAGE + (2 * BN + BM) * 4;
+    static constexpr int SLICES = BK / 32, STAGE = ROWS * BK;
+    static constexpr int BOX_LD = FN * 32 + 4, BOX = 32 * BOX_LD * 4;       // a wave's 32 tokens on their way out
+    static constexpr int TILES = S * STAGE > WAVES * BOX ? S * STAGE : WAVES * BOX, LDS = TILES + (2 * BN + BM) * 4;
     static_assert(ROWS % (PIECE_ROWS * WAVES) == 0 && LDS <= 160 * 1024 && (BK == 64 || BK == 128), "tile");
     static __device__ __forceinline__ int place(int row, int piece) { return (piece ^ ((row / (256 / BK)) & (PER_ROW - 1))) * 16; }
 };
@@ -296,7 +333,7 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
     };
 
     // the tile's scales and bias wait behind the tiles: at the end a lane needs 4 FN channels' and FM tokens'
-    float *sw = (float*)(smem + S * T::STAGE), *bias = sw + T::BN, *sa = bias + T::BN;
+    float *sw = (float*)(smem + T::TILES), *bias = sw + T::BN, *sa = bias + T::BN;
     for (int c = threadIdx.x; c < T::BN; c += T::THREADS) { sw[c] = i8_channel(p.sw, n0 + c, p.N); bias[c] = i8_channel(p.bias, n0 + c, p.N); }
     for (int c = threadIdx.x; c < T::BM; c += T::THREADS) sa[c] = i8_channel(p.sa, m0 + c, p.M);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");          // (the loop counts the loads that are under way)
@@ -371,37 +408,26 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
             multiply(0, 0, 0);
         }
     }
-    if (p.partial != nullptr) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FM; ++j) {
-                const int m = m0 + (wm * FM + j) * 32 + l31;
-                if (m >= p.M) continue;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int n = n0 + (wn * FN + i) * 32 + 8 * g + 4 * half;
-                    int* o = p.partial + ((size_t)blockIdx.y * p.M + m) * p.N + n;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = acc[i][j][4 * g + e];
-                }
-            }
-        return;
-    }
+    // A wave's 32 tokens at a time go through its own part of shared memory, so that its stores are whole lines of a token's row, whatever the
+    // row's alignment: a lane's accumulators lie 32 tokens apart.
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    int* box = (int*)(smem + wave * T::BOX);
+    const int nw = wn * FN * 32;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-        const int mt = (wm * FM + j) * 32 + l31, m = m0 + mt;
-        const float s = sa[mt];
-        if (m >= p.M) continue;
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int nt = (wn * FN + i) * 32 + 8 * g + 4 * half;
-                if (n0 + nt >= p.N) continue;
-                const int c[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                i8_store4(p, m, n0 + nt, c, s, *(const float4*)(sw + nt), *(const float4*)(bias + nt));
+                const intx4 c = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                *(intx4*)(box + l31 * T::BOX_LD + i * 32 + 8 * g + 4 * half) = c;
             }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int mt = (wm * FM + j) * 32;
+        const int rows = min(32, p.M - m0 - mt), cols = min(FN * 32, p.N - n0 - nw);
+        if (rows > 0 && cols > 0) i8_rows<FN * 32>(p, box, T::BOX_LD, m0 + mt, n0 + nw, rows, cols, sa + mt, sw + nw, bias + nw, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -411,16 +437,13 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)p.M * quads) return;
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    intx4 acc = {0, 0, 0, 0};
+    for (int s = 0; s < slices; ++s) acc += *(const intx4*)(p.partial + ((size_t)s * p.M + m) * (quads * 4) + n);
     const float sa = p.sa[m];
-    const float4 sw = make_float4(i8_channel(p.sw, n, p.N), i8_channel(p.sw, n + 1, p.N), i8_channel(p.sw, n + 2, p.N), i8_channel(p.sw, n + 3, p.N));
-    const float4 bias = make_float4(i8_channel(p.bias, n, p.N), i8_channel(p.bias, n + 1, p.N), i8_channel(p.bias, n + 2, p.N), i8_channel(p.bias, n + 3, p.N));
-    int acc[4] = {0, 0, 0, 0};
-    for (int s = 0; s < slices; ++s) {
-        const int* o = p.partial + ((size_t)s * p.M + m) * p.N + n;
+    float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += n + e < p.N ? o[e] : 0;
-    }
-    i8_store4(p, m, n, acc, sa, sw, bias);
+    for (int j = 0; j < 4; ++j) y[j] = i8_value(p, acc[j], sa, i8_channel(p.sw, n + j, p.N), i8_channel(p.bias, n + j, p.N));
+    i8_store4(p, (size_t)m * p.ldy + n, min(4, p.N - n), y);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ choice
