@@ -1426,8 +1426,14 @@ size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K) {
 int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                     int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream) {
     fbhip_ctx* none = nullptr;
-    RC(check_i8("fbhip_linear_i8", x, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, 1));
+    RC(check_i8("fbhip_linear_i8", x, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, 0));
     if (ldx < K || x_type < FBHIP_F32 || x_type > FBHIP_F16) { g_err = "fbhip_linear_i8: ldx < K or unknown input type"; return FBHIP_E_INVALID; }
+    if (linear_i8_fused(x, ldx, x_type, M, K)) {
+        I8Problem p{nullptr, w, nullptr, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, 0, ldw, ldy};
+        HIPCK(none, launch_linear_i8_tokens(p, x, ldx, x_type, (hipStream_t)stream));
+        return FBHIP_OK;
+    }
+    if (!workspace || ((uintptr_t)workspace & 15)) { g_err = "fbhip_linear_i8: workspace missing or not 16-byte aligned"; return FBHIP_E_INVALID; }
     size_t scale_at, rest_at;
     i8_carve(M, K, &scale_at, &rest_at);
     int8_t* codes = (int8_t*)workspace;

@@ -52,6 +52,30 @@ __device__ __forceinline__ I8Row i8_row(float top, bool bad) {
 
 __device__ __forceinline__ bool i8_no_number(float x) { return !(fabsf(x) < __uint_as_float(0x7F800000u)); }
 
+// values e of a 16-byte piece
+template <bool WIDE>
+__device__ __forceinline__ float i8_unpack(const uint32_t (&w)[4], int e, int type) {
+    if (WIDE) return __uint_as_float(w[e & 3]);
+    if (type == FBHIP_BF16) return __uint_as_float((e & 1) ? w[(e >> 1) & 3] & 0xFFFF0000u : w[(e >> 1) & 3] << 16);
+    const uint16_t h = (uint16_t)(w[(e >> 1) & 3] >> (16 * (e & 1)));
+    _Float16 g;
+    __builtin_memcpy(&g, &h, 2);
+    return (float)g;
+}
+
+// the piece at element k of a row of K: zero behind its end
+template <bool WIDE>
+__device__ __forceinline__ uint4 i8_piece(const char* base, int k, int K) {
+    constexpr int V = WIDE ? 4 : 8;
+    if (k + V <= K) return *(const uint4*)(base + (size_t)k * (16 / V));
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    for (int e = 0; e < K - k; ++e) {
+        if (WIDE) w[e] = ((const uint32_t*)base)[k + e];
+        else w[e >> 1] |= (uint32_t)((const uint16_t*)base)[k + e] << (16 * (e & 1));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A row in the registers of TPR threads: C pieces of 16 bytes a thread, read once.  Rows on 16-byte boundaries, K in whole pieces or not.
 // (One thread row of 64 takes up to 8 pieces: 2048 fp32 or 4096 16-bit values; a workgroup of 256 four times that.)
 template <int TPR, int C, bool WIDE>
@@ -69,32 +93,14 @@ __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __re
     uint4 raw[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int k = (c * TPR + t) * V;
-        raw[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (k + V <= K) raw[c] = *(const uint4*)(base + (size_t)k * (16 / V));
-        else if (k < K) {                                 // the piece that the row ends in
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-            for (int e = 0; e < K - k; ++e) {
-                if (WIDE) w[e] = ((const uint32_t*)base)[k + e];
-                else w[e >> 1] |= (uint32_t)((const uint16_t*)base)[k + e] << (16 * (e & 1));
-            }
-            raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        raw[c] = i8_piece<WIDE>(base, (c * TPR + t) * V, K);
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            float f;
-            if (WIDE) f = __uint_as_float(w[e & 3]);
-            else if (type == FBHIP_BF16) f = __uint_as_float((e & 1) ? w[(e >> 1) & 3] & 0xFFFF0000u : w[(e >> 1) & 3] << 16);
-            else {
-                const uint16_t h = (uint16_t)(w[(e >> 1) & 3] >> (16 * (e & 1)));
-                _Float16 g;
-                __builtin_memcpy(&g, &h, 2);
-                f = (float)g;
-            }
+            const float f = i8_unpack<WIDE>(w, e, type);
             v[c][e] = f;
             odd = odd || i8_no_number(f);
             top = fmaxf(top, fabsf(f));
@@ -446,6 +452,149 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
     i8_store4(p, (size_t)m * p.ldy + n, min(4, p.N - n), y);
 }
 
+// ------------------------------------------------------------------------------------------------------------------ few tokens
+// Few tokens: what counts is the weights' way from memory.  A workgroup of eight waves takes 16 NT channels and up to 16 MT tokens, its waves 128
+// codes of K in turn, both operands straight from memory into the 16x16x64 matrix instruction (a lane's 32 codes in a row are two
+// instructions' share: the operands agree on the order of K, which is all that the sum asks for).  The eight partial sums are added in shared memory.
+// TOKENS > 0: up to that many tokens are quantised by every workgroup for itself, while its first weights are on their way: a launch less.
+constexpr int I8_STRIP_WAVES = 8, I8_STRIP_THREADS = 64 * I8_STRIP_WAVES, I8_STRIP_PIECES = 4;
+
+// TOKENS rows of x into codes [TOKENS][Kp] and scales in shared memory; 512 / TOKENS threads a row
+template <int TOKENS, bool WIDE>
+__device__ __forceinline__ void i8_strip_quantize(const I8Problem& p, const void* x, int64_t ldx, int type, int8_t* codes, int Kp, float* scale, float* red,
+                                                  int* reds) {
+    constexpr int V = WIDE ? 4 : 8, TPT = I8_STRIP_THREADS / TOKENS, WPT = TPT / 64;
+    const int tid = threadIdx.x, m = tid / TPT, t = tid % TPT, wave = tid >> 6;
+    const char* base = (const char*)x + (size_t)min(m, p.M - 1) * ldx * (16 / V);
+    uint4 raw[I8_STRIP_PIECES];
+    float top = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < I8_STRIP_PIECES; ++c) raw[c] = i8_piece<WIDE>(base, (c * TPT + t) * V, p.K);
+#pragma unroll
+    for (int c = 0; c < I8_STRIP_PIECES; ++c) {
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float f = i8_unpack<WIDE>(w, e, type);
+            odd = odd || i8_no_number(f);
+            top = fmaxf(top, fabsf(f));
+        }
+    }
+    top = wave_max(top);
+    const int bad = __any(odd);
+    if ((tid & 63) == 0) { red[wave] = top; reds[wave] = bad; }
+    __syncthreads();
+    float all = 0.f;
+    int any = 0;
+#pragma unroll
+    for (int q = 0; q < WPT; ++q) { all = fmaxf(all, red[m * WPT + q]); any |= reds[m * WPT + q]; }
+    const I8Row r = i8_row(all, any != 0);
+    if (t == 0) scale[m] = r.scale;
+#pragma unroll
+    for (int c = 0; c < I8_STRIP_PIECES; ++c) {
+        const int k = (c * TPT + t) * V;
+        if (k >= Kp) break;
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+        uint32_t o[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e >> 2] |= (uint32_t)((r.zero ? 0 : i8_code(i8_unpack<WIDE>(w, e, type), r.scale, r.inv)) & 0xFF) << (8 * (e & 3));
+        if (WIDE) *(uint32_t*)(codes + m * Kp + k) = o[0];
+        else *(uint2*)(codes + m * Kp + k) = make_uint2(o[0], o[1]);
+    }
+    __syncthreads();
+}
+
+template <int NT, int MT, int TOKENS>
+__global__ void __launch_bounds__(I8_STRIP_THREADS) gemm_i8_strip_kernel(const I8Problem p, const void* __restrict__ x, int64_t ldx, int xtype) {
+    static_assert(TOKENS <= 16 && (TOKENS == 0 || MT == 1), "quantised tokens fit one tile");
+    extern __shared__ __attribute__((aligned(16))) int8_t codes[];         // TOKENS > 0: [TOKENS][Kp]
+    __shared__ __attribute__((aligned(16))) intx4 part[I8_STRIP_WAVES][NT * MT][64];
+    __shared__ float token_scale[16], red[I8_STRIP_WAVES];
+    __shared__ int reds[I8_STRIP_WAVES];
+    constexpr int DEEP = NT * MT >= 4 ? 2 : 4;                // chunks whose loads are under way together
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, quarter = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT, K = p.K, chunks = (K + 127) / 128, k16 = (K + 15) & ~15, Kp = chunks * 128;
+    const int8_t *wp[NT], *ap[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wp[i] = p.w + (size_t)min(n0 + 16 * i + l15, p.N - 1) * p.ldw;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) ap[j] = TOKENS ? codes + l15 * Kp : p.a + (size_t)min(m0 + 16 * j + l15, p.M - 1) * p.lda;
+    intx4 acc[NT][MT], w[DEEP][NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+    auto load = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            if (c0 + d * I8_STRIP_WAVES >= chunks) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = min((c0 + d * I8_STRIP_WAVES) * 128 + quarter * 32 + h * 16, k16 - 16);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) w[d][i][h] = *(const intx4*)(wp[i] + k);
+            }
+        }
+    };
+    load(wave);
+    if (TOKENS) {
+        if (xtype == FBHIP_F32) i8_strip_quantize<TOKENS ? TOKENS : 1, true>(p, x, ldx, xtype, codes, Kp, token_scale, red, reds);
+        else i8_strip_quantize<TOKENS ? TOKENS : 1, false>(p, x, ldx, xtype, codes, Kp, token_scale, red, reds);
+    }
+    for (int c0 = wave; c0 < chunks; c0 += I8_STRIP_WAVES * DEEP) {
+        intx4 a[DEEP][MT][2];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int c = c0 + d * I8_STRIP_WAVES;
+            if (c >= chunks) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = c * 128 + quarter * 32 + h * 16;
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    if (TOKENS) a[d][j][h] = l15 < TOKENS ? *(const intx4*)(ap[j] + k) : intx4{0, 0, 0, 0};
+                    else a[d][j][h] = *(const intx4*)(ap[j] + min(k, k16 - 16));
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int c = c0 + d * I8_STRIP_WAVES;
+            if (c >= chunks) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!TOKENS && c == chunks - 1 && (K & 127)) {          // codes behind K count nothing, whatever the weights hold there
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) a[d][j][h] = i8_mask(a[d][j][h], K - (c * 128 + quarter * 32 + h * 16));
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][i][h], a[d][j][h], acc[i][j], 0, 0, 0);
+            }
+        }
+        if (c0 + I8_STRIP_WAVES * DEEP < chunks) load(c0 + I8_STRIP_WAVES * DEEP);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) part[wave][i * MT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int q = threadIdx.x; q < NT * MT * 64; q += I8_STRIP_THREADS) {
+        const int f = q >> 6, l = q & 63, m = m0 + 16 * (f % MT) + (l & 15), n = n0 + 16 * (f / MT) + 4 * (l >> 4);
+        if (m >= p.M || n >= p.N) continue;
+        intx4 v = part[0][f][l];
+#pragma unroll
+        for (int u = 1; u < I8_STRIP_WAVES; ++u) v += part[u][f][l];
+        const float sa = TOKENS ? token_scale[m] : p.sa[m];
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = i8_value(p, v[e], sa, i8_channel(p.sw, n + e, p.N), i8_channel(p.bias, n + e, p.N));
+        i8_store4(p, (size_t)m * p.ldy + n, min(4, p.N - n), y);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------ choice
 template <int WN, int WM, int FN, int FM, int BK, int S>
 static hipError_t launch_i8_tile(I8Problem p, int slices, hipStream_t s) {
@@ -459,12 +608,16 @@ static hipError_t launch_i8_tile(I8Problem p, int slices, hipStream_t s) {
     return hipGetLastError();
 }
 
+constexpr int I8_STRIP_TOKENS = 64;
+
 I8Plan gemm_i8_plan(int M, int N, int K) {
     I8Plan plan{};
     const int steps = (K + I8_BK - 1) / I8_BK;
+    plan.slices = 1;
+    plan.steps = steps;
+    if (M <= I8_STRIP_TOKENS) { plan.tile = 16; return plan; }
     const int64_t t256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256), t128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
     const int64_t t64 = (int64_t)((M + 63) / 64) * ((N + 63) / 64);
-    plan.slices = 1;
     if (t256 >= 192) plan.tile = 256;
     else if (t128 >= 192) plan.tile = 128;
     else {
@@ -478,12 +631,49 @@ I8Plan gemm_i8_plan(int M, int N, int K) {
     return plan;
 }
 
-hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
-    const I8Plan plan = gemm_i8_plan(p.M, p.N, p.K);
-    p.steps = plan.steps;
-    p.partial = plan.slices > 1 ? partial : nullptr;
+static void i8_output(I8Problem& p) {
     const size_t size = p.ytype == FBHIP_F32 ? 4 : 2;
     p.yvec = ((uintptr_t)p.y % (4 * size) == 0) && p.ldy % 4 == 0;
+}
+
+template <int NT, int MT>
+static void launch_i8_strip(const I8Problem& p, hipStream_t s) {
+    hipLaunchKernelGGL((gemm_i8_strip_kernel<NT, MT, 0>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(I8_STRIP_THREADS), 0, s, p,
+                       nullptr, (int64_t)0, (int)FBHIP_F32);
+}
+
+template <int TOKENS>
+static void launch_i8_strip_tokens(const I8Problem& p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
+    const size_t lds = (size_t)TOKENS * ((p.K + 127) / 128 * 128);
+    hipLaunchKernelGGL((gemm_i8_strip_kernel<1, 1, TOKENS>), dim3((p.N + 15) / 16), dim3(I8_STRIP_THREADS), lds, s, p, x, ldx, xtype);
+}
+
+// Up to four tokens whose values fit four pieces of 16 bytes a thread, on 16-byte rows.
+bool linear_i8_fused(const void* x, int64_t ldx, int xtype, int M, int K) {
+    const int V = xtype == FBHIP_F32 ? 4 : 8, rows = M == 3 ? 4 : M;
+    return M <= 4 && ((uintptr_t)x & 15) == 0 && (M == 1 || (ldx * (16 / V)) % 16 == 0) && (K + 127) / 128 * 128 <= I8_STRIP_THREADS / rows * V * I8_STRIP_PIECES;
+}
+
+hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
+    i8_output(p);
+    if (p.M == 1) launch_i8_strip_tokens<1>(p, x, ldx, xtype, s);
+    else if (p.M == 2) launch_i8_strip_tokens<2>(p, x, ldx, xtype, s);
+    else launch_i8_strip_tokens<4>(p, x, ldx, xtype, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
+    const I8Plan plan = gemm_i8_plan(p.M, p.N, p.K);
+    i8_output(p);
+    if (plan.tile == 16) {
+        const bool wide = p.N >= 8192;
+        if (p.M <= 16) launch_i8_strip<1, 1>(p, s);
+        else if (p.M <= 32) wide ? launch_i8_strip<2, 2>(p, s) : launch_i8_strip<1, 2>(p, s);
+        else wide ? launch_i8_strip<2, 4>(p, s) : launch_i8_strip<1, 4>(p, s);
+        return hipGetLastError();
+    }
+    p.steps = plan.steps;
+    p.partial = plan.slices > 1 ? partial : nullptr;
     hipError_t e;
     if (plan.tile == 256) e = launch_i8_tile<4, 4, 2, 2, 128, 2>(p, plan.slices, s);
     else if (plan.tile == 128) e = launch_i8_tile<2, 4, 2, 1, 128, 2>(p, plan.slices, s);

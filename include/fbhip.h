@@ -525,7 +525,7 @@ int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* code
                         int32_t Kp, void* stream);
 /* y[m, n] = act((sum_k a[m, k] w[n, k]) * a_scale[m] * w_scale[n] + bias[n]).  a, w: 8-bit codes, rows on 16-byte boundaries and readable to the
  * next multiple of 16 (what lies behind K does not count).  bias nullable; relu: 0 / 1; y: FBHIP_F32 / BF16 / F16, rows ldy elements apart.
- * workspace: fbhip_gemm_i8_workspace bytes (16-byte aligned; nullable where that is 0). */
+ * workspace: fbhip_gemm_i8_workspace / fbhip_linear_i8_workspace bytes (16-byte aligned; nullable where that is 0). */
 size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K);
 int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                   int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);

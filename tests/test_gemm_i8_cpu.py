@@ -47,23 +47,23 @@ def test_host_tensors_are_refused():
 
 def test_c_entries_refuse_bad_calls():
     lib = _lib.load()
-    ok = dict(a=16, lda=32, sa=16, w=16, ldw=32, sw=16, bias=None, relu=0, y=16, ldy=4, yt=0, M=4, N=4, K=20, ws=16)
+    ok = dict(a=16, lda=2000, sa=16, w=16, ldw=2000, sw=16, bias=None, relu=0, y=16, ldy=4, yt=0, M=400, N=4, K=2000, ws=16)
 
     def gemm(**kw):
         d = dict(ok, **kw)
         return lib.fbhip_gemm_i8(d["a"], d["lda"], d["sa"], d["w"], d["ldw"], d["sw"], d["bias"], d["relu"], d["y"], d["ldy"], d["yt"], d["M"], d["N"],
                                  d["K"], d["ws"], None)
     for kw in (dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(y=None), dict(M=0), dict(N=0), dict(K=0), dict(K=131073, lda=131088, ldw=131088),
-               dict(a=8), dict(w=8), dict(lda=20), dict(ldw=20), dict(lda=16), dict(ldw=16), dict(ldy=3), dict(yt=3), dict(yt=-1),
+               dict(a=8), dict(w=8), dict(lda=2004), dict(ldw=2004), dict(lda=1984), dict(ldw=1984), dict(ldy=3), dict(ws=None), dict(ws=8), dict(yt=3), dict(yt=-1),
                dict(ldw=1 << 24), dict(lda=1 << 24), dict(M=2 ** 31 - 1, N=2 ** 31 - 1, ldy=2 ** 31)):
         assert gemm(**kw) == -1 and lib.fbhip_last_error(None), kw
-    def lin(x=16, ldx=20, xt=0, ws=16, **kw):
+    def lin(x=16, ldx=2000, xt=0, ws=16, **kw):
         d = dict(ok, **kw)
         return lib.fbhip_linear_i8(x, ldx, xt, d["w"], d["ldw"], d["sw"], None, 0, d["y"], d["ldy"], d["yt"], d["M"], d["N"], d["K"], ws, None)
-    assert all(r == -1 for r in (lin(x=None), lin(ldx=19), lin(xt=3), lin(ws=None), lin(ws=8), lin(w=None), lin(K=0)))
+    assert all(r == -1 for r in (lin(x=None), lin(ldx=1999), lin(xt=3), lin(ws=None), lin(ws=8), lin(w=None), lin(K=0)))
 
     def quant(x=16, ldx=20, xt=0, q=16, ldq=32, s=16, rows=4, k=20, kp=32):
         return lib.fbhip_quantize_rows(x, ldx, xt, q, ldq, s, rows, k, kp, None)
     assert all(r == -1 for r in (quant(x=None), quant(q=None), quant(s=None), quant(rows=0), quant(k=0), quant(kp=19), quant(ldq=31), quant(ldx=19),
                                  quant(xt=5)))
-    assert lib.fbhip_linear_i8_workspace(4, 4, 20) >= 4 * 128 + 16 and lib.fbhip_linear_i8_workspace(0, 4, 20) == 0
+    assert lib.fbhip_linear_i8_workspace(40, 4, 20) >= 40 * 128 + 160 and lib.fbhip_linear_i8_workspace(0, 4, 20) == 0

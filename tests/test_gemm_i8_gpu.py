@@ -43,7 +43,7 @@ def _check(y, a, sa, w, sw, bias, relu, dtype):
 
 
 # the tiles' borders (16, 32, 64, 128, 256) and their neighbours; one token; layers of the agents' networks; uneven K
-SIZES = [(1, 1, 1), (1, 6, 24), (1, 1024, 1024), (2, 50, 1024), (3, 17, 130), (4, 1000, 77), (5, 64, 128), (15, 16, 127), (16, 33, 129), (17, 526, 526), (31, 100, 256),
+SIZES = [(1, 1, 1), (1, 6, 24), (1, 1024, 1024), (2, 50, 1024), (2, 8200, 1500), (1, 20000, 70), (3, 17, 130), (4, 4100, 1025), (4, 300, 17000), (4, 1000, 77), (5, 64, 128), (15, 16, 127), (16, 33, 129), (17, 526, 526), (31, 100, 256),
          (33, 65, 97), (63, 63, 4096), (64, 64, 384), (65, 70, 1000), (64, 6, 8191), (127, 129, 255), (128, 128, 512), (200, 300, 1051), (256, 256, 128), (257, 255, 640),
          (300, 1024, 74), (777, 526, 1051), (1000, 2048, 1024), (1024, 2048, 30), (2500, 1300, 333)]
 
@@ -162,7 +162,7 @@ def test_rows_that_hold_no_numbers(K, M, bad):
 # ------------------------------------------------------------------------------------------------------------------------------ linear
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 16, 17, 48, 64, 65, 300])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("N,Kd", [(6, 30), (526, 1051), (1024, 1024), (64, 8200)])
+@pytest.mark.parametrize("N,Kd", [(6, 30), (526, 1051), (1024, 1024), (64, 8200), (40, 33000)])
 def test_linear_equals_quantize_then_product(K, M, N, Kd, dtype):
     gen = torch.Generator().manual_seed(M + N)
     x = torch.randn(M, Kd, generator=gen).to(dtype).cuda()
