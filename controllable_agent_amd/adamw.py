@@ -6,8 +6,10 @@ global gradient norm, and moments that take 2 bytes a parameter instead of 8.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
+import operator
 import typing as tp
 
 import torch
@@ -18,6 +20,8 @@ from ._lib import check
 BLOCK = 256            # elements that share a scale of an 8-bit moment
 CHUNK = 2048           # FBHIP_ADAMW_CHUNK
 GRAD_DENSE = 4         # FBHIP_GRAD_DENSE
+CONTROL_BYTES = 2304   # FBHIP_ADAMW_CONTROL_BYTES
+_SHAPE_TYPE_DEVICE = operator.attrgetter("shape", "dtype", "device")
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -74,8 +78,8 @@ class AdamW:
             raise ValueError("AdamW: no parameters")
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
-        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and 0.0 <= eps < math.inf):
-            raise ValueError(f"AdamW: 0 <= beta < 1 and eps >= 0, got betas={betas}, eps={eps}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and (eps == 0.0 or 1e-30 <= eps < math.inf)):
+            raise ValueError(f"AdamW: 0 <= beta < 1 and eps 0 or at least 1e-30, got betas={betas}, eps={eps}")
         wd, scale = _per_tensor("weight_decay", weight_decay, n), _per_tensor("lr_scale", lr_scale, n)
         self._layouts: tp.List[tp.Tuple[int, int]] = []          # (cols, ld); cols 0: dense
         spans = []
@@ -128,7 +132,7 @@ class AdamW:
         else:
             self.m8, self.r8 = zeros(size, torch.uint8).view(torch.float8_e4m3fn), zeros(size, torch.uint8).view(torch.float8_e4m3fn)
             self.m_scale, self.r_scale = zeros(size // BLOCK, torch.float32), zeros(size // BLOCK, torch.float32)
-        self._control = zeros(8, torch.int64)                    # FBHIP_ADAMW_CONTROL_BYTES
+        self._control = zeros(CONTROL_BYTES // 8, torch.int64)
         self._norm = self._control.view(torch.float32)[6]        # byte 24
         self._partials = zeros(_lib.load().fbhip_adamw_partials(n), torch.float64)
         m, v = (self.m, self.v) if state_bits == 32 else (self.m8, self.r8)
@@ -136,8 +140,10 @@ class AdamW:
                          m.data_ptr(), v.data_ptr(), None if state_bits == 32 else self.m_scale.data_ptr(),
                          None if state_bits == 32 else self.r_scale.data_ptr(), self._control.data_ptr(), self._partials.data_ptr(),
                          *self.betas, self.eps)
-        self._shapes, self._strides = [p.shape for p in self.params], [p.stride() for p in self.params]
-        self._grad_array, self._type_array = C.c_void_p * n, C.c_uint8 * n
+        self._opt_ref = C.byref(self._opt)
+        self._seen: tp.Any = None
+        self._seen_strides: tp.Any = None
+        self._types = b""
         self._set_step(0)
 
     def _interleaved(self, i: int, j: int) -> bool:
@@ -152,29 +158,33 @@ class AdamW:
         with torch.cuda.device(self.device):
             check(_lib.load().fbhip_adamw_set_step(C.byref(self._opt), int(step), torch.cuda.current_stream().cuda_stream))
 
-    def _grad_types(self, grads: tp.List[torch.Tensor]) -> tp.List[int]:
+    def _grad_types(self, grads: tp.List[torch.Tensor]) -> bytes:
+        """the type of each gradient for the kernel, after the checks that its place beside the parameters needs"""
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} parameters")
-        if any(g is None for g in grads):
-            raise ValueError("AdamW.step: a gradient is None: leave its parameter out, or pass zeros (which decay its moments)")
         try:
-            types = [_TYPES[g.dtype] for g in grads]
-        except KeyError as e:
-            raise TypeError(f"AdamW.step: gradients are float32, bfloat16 or float16, got {e}") from None
-        if [g.shape for g in grads] != self._shapes:
-            raise ValueError("AdamW.step: a gradient's shape is not its parameter's")
-        if any(g.device != self.device for g in grads):
-            raise ValueError(f"AdamW.step: gradients on {self.device} expected")
-        if [g.stride() for g in grads] != self._strides:
-            for k, (g, p) in enumerate(zip(grads, self.params)):
-                cols = self._layouts[k][0]
-                if g.stride() == self._strides[k] or (not cols and p.is_contiguous() and g.is_contiguous()):
-                    continue
+            seen = list(map(_SHAPE_TYPE_DEVICE, grads))
+            strides = list(map(torch.Tensor.stride, grads))
+        except (AttributeError, TypeError):
+            raise ValueError("AdamW.step: a gradient is no tensor: leave its parameter out, or pass zeros (which decay its moments)") from None
+        if seen == self._seen and strides == self._seen_strides:        # shapes, types, devices and strides as in the last step
+            return self._types
+        types = bytearray()
+        for k, (g, p) in enumerate(zip(grads, self.params)):
+            if g.dtype not in _TYPES:
+                raise TypeError(f"AdamW.step: gradients are float32, bfloat16 or float16, got {g.dtype}")
+            if g.shape != p.shape or g.device != self.device:
+                raise ValueError(f"AdamW.step: gradient {k} is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {self.device}")
+            cols = self._layouts[k][0]
+            flag = 0
+            if g.stride() != p.stride() and not (not cols and p.is_contiguous() and g.is_contiguous()):
                 if not (cols and g.is_contiguous()):
-                    raise ValueError(f"AdamW.step: gradient {k} has strides {g.stride()}, its parameter {self._strides[k]}: the same, or a "
+                    raise ValueError(f"AdamW.step: gradient {k} has strides {g.stride()}, its parameter {p.stride()}: the same, or a "
                                      "contiguous gradient of a row-strided matrix, expected")
-                types[k] |= GRAD_DENSE
-        return types
+                flag = GRAD_DENSE
+            types.append(_TYPES[g.dtype] | flag)
+        self._seen, self._seen_strides, self._types = seen, strides, bytes(types)
+        return self._types
 
     @torch.no_grad()
     def step(self, grads: tp.Sequence[torch.Tensor], *, lr: tp.Union[float, torch.Tensor, None] = None, grad_scale: float = 1.0,
@@ -198,8 +208,9 @@ class AdamW:
             lr_value = float(lr)
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"AdamW.step: max_norm > 0 expected, got {max_norm}")
-        args = (C.byref(self._opt), self._grad_array(*[g.data_ptr() or None for g in grads]), self._type_array(*types), lr_ptr, lr_value,
-                float(grad_scale), int(max_norm is not None), 0.0 if max_norm is None else float(max_norm))
+        pointers = array.array("Q", map(torch.Tensor.data_ptr, grads))
+        args = (self._opt_ref, pointers.buffer_info()[0], types, lr_ptr, lr_value, float(grad_scale), int(max_norm is not None),
+                0.0 if max_norm is None else float(max_norm))
         if torch.cuda.current_device() == self.device.index:
             check(_lib.load().fbhip_adamw_step(*args, torch.cuda.current_stream().cuda_stream))
         else:

@@ -27,15 +27,29 @@ constexpr int ADAMW_MAX_TENSORS = 384;       // gradient addresses travel in the
 constexpr int ADAMW_BLOCKS = 2048;           // eight workgroups for each of 256 CUs; they walk the chunks
 constexpr int ADAMW_NORM_BLOCKS = 1024;      // one partial sum each, folded in order
 
+// Workgroups count themselves off in 32 groups: 2048 additions to one address take 20 us, in turn, at the end of a step that takes 40.
+constexpr int ADAMW_GROUPS = 32;
+
 // The optimiser's scalars on the device (FBHIP_ADAMW_CONTROL_BYTES): a replayed graph advances them.
 struct AdamwControl {
     int64_t t;                               // steps done
     double b1t, b2t;                         // b1^t, b2^t
-    float norm, gs;                          // of this step, where it clips
-    int32_t skip;                            // the norm is not finite: the step changes nothing
-    uint32_t step_ticket, norm_ticket;
+    float norm;                              // of the gradients of the last step that clipped
+    uint32_t root;                           // groups of workgroups that are done
+    uint32_t pad[5];
+    uint32_t group[ADAMW_GROUPS][16];        // workgroups that are done, on a line of their own for each group
 };
 static_assert(sizeof(AdamwControl) <= FBHIP_ADAMW_CONTROL_BYTES, "control block");
+
+// The tables do not change while a kernel runs: scalar loads may read them.
+template <class T>
+__device__ __forceinline__ T table(const T* base, int i) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return ((const T __attribute__((address_space(4)))*)(uintptr_t)base)[i];
+#else
+    return base[i];          // (the host pass has no such address space; it never runs this)
+#endif
+}
 
 struct AdamwArgs {
     const fbhip_adamw_tensor* tensors;
@@ -49,7 +63,9 @@ struct AdamwArgs {
     float *m_scale, *r_scale;
     double lr, b1, b2;
     const float* lr_ptr;
-    float eps, grad_scale;
+    const double* partial;                   // of the gradients' squares
+    int partials;
+    float eps, grad_scale, max_norm;
     uint32_t seed;
     const void* grad[ADAMW_MAX_TENSORS];
     uint8_t gtype[ADAMW_MAX_TENSORS];
@@ -60,10 +76,7 @@ struct NormArgs {
     const fbhip_adamw_tensor* tensors;
     const int2* chunks;
     int first, last, tensor0;
-    int partial0, partials;                  // this launch's first partial sum, and how many there are in the last launch (else 0)
-    double* partial;
-    AdamwControl* ctl;
-    float max_norm, grad_scale;
+    double* partial;                         // one for each workgroup
     const void* grad[ADAMW_MAX_TENSORS];
     uint8_t gtype[ADAMW_MAX_TENSORS];
 };
@@ -126,22 +139,32 @@ __device__ __forceinline__ uint32_t finish_word(uint32_t h) {
     h = (h ^ (h >> 13)) * 0xC2B2AE35u;
     return h ^ (h >> 16);
 }
-__device__ __forceinline__ uint32_t element_word(int64_t i, uint32_t key) {
-    // places beyond 2^32 take a key of their own
-    return finish_word((uint32_t)i * 0x9E3779B1u + key + (uint32_t)((uint64_t)i >> 32) * 0x27D4EB2Fu);
+// of the eight elements from place i on; places beyond 2^32 take a key of their own (i is a multiple of eight: none of them crosses over)
+__device__ __forceinline__ void element_words(int64_t i, uint32_t key, uint32_t (&w)[8]) {
+    const uint32_t first = (uint32_t)i * 0x9E3779B1u + key + (uint32_t)((uint64_t)i >> 32) * 0x27D4EB2Fu;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) w[j] = finish_word(first + j * 0x9E3779B1u);
 }
 
 // e4m3 codes of eight lane values and the block's scale (half a wave = 256 elements); u: 16 random bits for each value
 template <bool POSITIVE>
 __device__ __forceinline__ uint2 encode_eight(const float (&x)[8], const uint32_t (&u)[8], float& scale) {
-    uint32_t top = 0;
+    uint32_t mag[8], top = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
-        top = max(top, b < 0x7F800000u ? b : 0u);
+        mag[j] = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+        top = max(top, mag[j]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    const bool odd = top >= 0x7F800000u;          // somewhere in the block something is no number: it does not count for the scale
+    if (odd) {
+        top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, mag[j] < 0x7F800000u ? mag[j] : 0u);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    }
     // 448 = 1.75 * 2^8: the exponent field of 2^k with top * 2^-k <= 448; at least 1, so that 2^k and 2^-k are normal numbers
     const int field = max((int)((top + 0x1FFFFFu) >> 23) - 8, 1);
     scale = __uint_as_float((uint32_t)field << 23);
@@ -149,15 +172,18 @@ __device__ __forceinline__ uint2 encode_eight(const float (&x)[8], const uint32_
     uint32_t c[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(x[j]), mag = b & 0x7FFFFFFFu;
-        const float y = __uint_as_float(mag) * inv;
+        const float y = __uint_as_float(mag[j]) * inv;
         // three mantissa bits stay; below 2^-6 the codes are evenly spaced, which adding 2^-6 brings about
         const bool small = y < 0.015625f;
         const uint32_t z = __float_as_uint(small ? y + 0.015625f : y);
-        int code = (int)((z + (u[j] << 4)) >> 20) - (small ? 968 : 960);
-        if (POSITIVE) code = (code == 0 && mag != 0) ? 1 : code;
-        code = mag < 0x7F800000u ? code : 0x7F;
-        c[j] = (uint32_t)code | (POSITIVE ? 0u : (b >> 24) & 0x80u);
+        c[j] = ((u[j] << 4) + z - (small ? 968u << 20 : 960u << 20)) >> 20;
+        if (POSITIVE) c[j] = max(c[j], min(mag[j], 1u));
+        else c[j] |= (__float_as_uint(x[j]) >> 24) & 0x80u;
+    }
+    if (odd) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (mag[j] >= 0x7F800000u) c[j] = 0x7Fu | (POSITIVE ? 0u : (__float_as_uint(x[j]) >> 24) & 0x80u);
     }
     return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
 }
@@ -169,42 +195,47 @@ __device__ __forceinline__ void decode_eight(uint2 q, float scale, float (&x)[8]
     x[4] = c[0] * scale; x[5] = c[1] * scale; x[6] = d[0] * scale; x[7] = d[1] * scale;
 }
 
+// lanes and waves folded in a fixed order
+__device__ __forceinline__ double block_sum(double x, double* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
 template <int BITS>
 __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a) {
 #pragma clang fp contract(off)
-    __shared__ double shared_lr, shared_ibc1;
+    __shared__ double red[4], shared_lr, shared_ibc1;
     __shared__ float shared_rbc2, shared_gs;
     __shared__ uint32_t shared_key;
     const int tid = threadIdx.x;
+    float norm = 0.f;
+    if (a.clip) {
+        // every workgroup adds the partial sums for itself, in the same order
+        double x = 0.0;
+        for (int k = tid; k < a.partials; k += ADAMW_THREADS) x += a.partial[k];
+        norm = (float)(fabs((double)a.grad_scale) * sqrt(block_sum(x, red)));
+        if (blockIdx.x == 0 && tid == 0 && a.advance) a.ctl->norm = norm;
+        if (!(norm < __uint_as_float(0x7F800000u))) return;          // not a number: nothing changes, nothing counts
+    }
     if (tid == 0) {
-        const AdamwControl c = *a.ctl;
-        const double b1t = c.b1t * a.b1, b2t = c.b2t * a.b2;
+        const double b1t = a.ctl->b1t * a.b1, b2t = a.ctl->b2t * a.b2;
         shared_lr = a.lr_ptr != nullptr ? (double)*a.lr_ptr : a.lr;
         shared_ibc1 = 1.0 / (1.0 - b1t);
         shared_rbc2 = (float)(1.0 / sqrt(1.0 - b2t));
-        shared_gs = a.clip ? c.gs : a.grad_scale;
-        shared_key = finish_word(a.seed ^ (uint32_t)(c.t + 1) * 0x27D4EB2Fu);
-        const bool skip = a.clip && c.skip;
-        if (skip) shared_gs = __uint_as_float(0x7FC00000u);
-        if (a.advance && !skip) {
-            // every workgroup has read the scalars when the last one comes here: it moves them to the next step
-            if (__hip_atomic_fetch_add(&a.ctl->step_ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
-                a.ctl->step_ticket = 0;
-                a.ctl->t = c.t + 1;
-                a.ctl->b1t = b1t;
-                a.ctl->b2t = b2t;
-            }
-        }
+        shared_gs = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.f);
+        shared_key = finish_word(a.seed ^ (uint32_t)(a.ctl->t + 1) * 0x27D4EB2Fu);
     }
     __syncthreads();
     const float gs = shared_gs, rbc2 = shared_rbc2, eps = a.eps;
-    if (a.clip && gs != gs) return;
     const double lr = shared_lr, ibc1 = shared_ibc1;
     const uint32_t key = shared_key;
     const float w1 = (float)(1.0 - a.b1), w2 = (float)(1.0 - a.b2), b2 = (float)a.b2;
     for (int c = a.first + (int)blockIdx.x; c < a.last; c += (int)gridDim.x) {
-        const int2 e = a.chunks[c];
-        const fbhip_adamw_tensor T = a.tensors[e.x];
+        const int2 e = table(a.chunks, c);
+        const fbhip_adamw_tensor T = table(a.tensors, e.x);
         const int64_t i = (int64_t)e.y * ADAMW_CHUNK + tid * ADAMW_PER_LANE;
         // the moments are padded to whole blocks of 256 for each tensor: half a wave is inside or outside as one
         if (i >= ((T.numel + 255) & ~(int64_t)255)) continue;
@@ -243,15 +274,26 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a)
             const float gr = g[j] * gs;
             m[j] = m[j] + w1 * (gr - m[j]);
             v[j] = v[j] * b2 + (w2 * gr) * gr;
-            r[j] = sqrtf(v[j]);
+        }
+        // The square root's instruction is good to one step, for normal numbers; so is the reciprocal's (the denominator is none or normal: the root of
+        // the least number is 3.7e-23)
+        uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            r[j] = __builtin_amdgcn_sqrtf(v[j]);
+            least = min(least, __float_as_uint(v[j]) - 1u);
+        }
+        if (least < 0x7FFFFFu) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = sqrtf(v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
             const float den = r[j] * rbc2 + eps;
-            p[j] = p[j] * keep - ss * (m[j] / den);
+            p[j] = p[j] * keep - ss * (m[j] * __builtin_amdgcn_rcpf(den));
         }
         uint32_t word[8];
-        if (BITS == 8 || T.dtype == FBHIP_BF16) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) word[j] = element_word(s + j, key);
-        }
+        if (BITS == 8 || T.dtype == FBHIP_BF16) element_words(s, key, word);
         if (BITS == 32) {
             *(float4*)((float*)a.m + s) = make_float4(m[0], m[1], m[2], m[3]);
             *(float4*)((float*)a.m + s + 4) = make_float4(m[4], m[5], m[6], m[7]);
@@ -299,55 +341,40 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a)
             }
         }
     }
+    if (tid != 0 || !a.advance) return;
+    // every workgroup has read the scalars when the last one comes here: it moves them to the next step
+    const uint32_t mine = blockIdx.x % ADAMW_GROUPS, members = (gridDim.x - mine + ADAMW_GROUPS - 1) / ADAMW_GROUPS;
+    if (__hip_atomic_fetch_add(&a.ctl->group[mine][0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != members - 1) return;
+    a.ctl->group[mine][0] = 0;
+    const uint32_t groups = gridDim.x < ADAMW_GROUPS ? gridDim.x : ADAMW_GROUPS;
+    if (__hip_atomic_fetch_add(&a.ctl->root, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != groups - 1) return;
+    a.ctl->root = 0;
+    a.ctl->t += 1;
+    a.ctl->b1t *= a.b1;
+    a.ctl->b2t *= a.b2;
 }
 
-// sum of squares in doubles (the square of the largest fp32 is far inside their range), lanes folded in a fixed tree
-__device__ __forceinline__ double block_sum(double x, double* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
-}
-
+// The squares are summed in doubles: the square of the largest fp32 is far inside their range.
 __global__ void __launch_bounds__(ADAMW_THREADS) adamw_norm_kernel(const NormArgs a) {
-    __shared__ double red[4], red2[4];
-    __shared__ int is_last;
-    const int tid = threadIdx.x;
+    __shared__ double red[4];
     double acc = 0.0;
     for (int c = a.first + (int)blockIdx.x; c < a.last; c += (int)gridDim.x) {
-        const int2 e = a.chunks[c];
-        const fbhip_adamw_tensor T = a.tensors[e.x];
+        const int2 e = table(a.chunks, c);
+        const fbhip_adamw_tensor T = table(a.tensors, e.x);
         float g[8];
-        load_grad(T, a.grad[e.x - a.tensor0], a.gtype[e.x - a.tensor0], (int64_t)e.y * ADAMW_CHUNK + tid * ADAMW_PER_LANE, g);
+        load_grad(T, a.grad[e.x - a.tensor0], a.gtype[e.x - a.tensor0], (int64_t)e.y * ADAMW_CHUNK + (int)threadIdx.x * ADAMW_PER_LANE, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc += (double)g[j] * (double)g[j];
     }
     const double sum = block_sum(acc, red);
-    if (tid == 0) {
-        __hip_atomic_store(a.partial + a.partial0 + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        is_last = a.partials > 0 &&
-                  __hip_atomic_fetch_add(&a.ctl->norm_ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-    }
-    __syncthreads();
-    if (!is_last) return;
-    double x = 0.0;
-    for (int k = tid; k < a.partials; k += ADAMW_THREADS)
-        x += __hip_atomic_load(a.partial + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const double total = block_sum(x, red2);
-    if (tid != 0) return;
-    const float norm = (float)(fabs((double)a.grad_scale) * sqrt(total));
-    const bool finite = norm < __uint_as_float(0x7F800000u);
-    a.ctl->norm_ticket = 0;
-    a.ctl->norm = norm;
-    a.ctl->skip = finite ? 0 : 1;
-    a.ctl->gs = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.f);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
 }
 
 __global__ void adamw_set_kernel(AdamwControl* c, int64_t t, double b1t, double b2t) {
     c->t = t; c->b1t = b1t; c->b2t = b2t;
-    c->norm = 0.f; c->gs = 1.f; c->skip = 0;
-    c->step_ticket = 0; c->norm_ticket = 0;
+    c->norm = 0.f;
+    c->root = 0;
+    for (int g = 0; g < ADAMW_GROUPS; ++g) c->group[g][0] = 0;
 }
 
 hipError_t launch_adamw_set(void* control, int64_t t, double b1, double b2, hipStream_t s) {
@@ -358,25 +385,23 @@ hipError_t launch_adamw_set(void* control, int64_t t, double b1, double b2, hipS
 hipError_t launch_adamw_step(const fbhip_adamw* o, const void* const* grads, const uint8_t* gtypes, const float* lr_ptr, double lr,
                              float grad_scale, int clip, float max_norm, hipStream_t s) {
     const int n = o->n_tensors, launches = (n + ADAMW_MAX_TENSORS - 1) / ADAMW_MAX_TENSORS;
+    int partials = 0;
     if (clip) {
         NormArgs a{};
         a.tensors = o->tensors; a.chunks = (const int2*)o->chunks;
-        a.partial = o->partials; a.ctl = (AdamwControl*)o->control;
-        a.max_norm = max_norm; a.grad_scale = grad_scale;
-        int done = 0;
         for (int l = 0; l < launches; ++l) {
             const int t0 = l * ADAMW_MAX_TENSORS, t1 = min(n, t0 + ADAMW_MAX_TENSORS);
             a.first = o->host_first_chunk[t0]; a.last = o->host_first_chunk[t1]; a.tensor0 = t0;
             for (int t = t0; t < t1; ++t) { a.grad[t - t0] = grads[t]; a.gtype[t - t0] = gtypes[t]; }
             const int blocks = max(1, min(ADAMW_NORM_BLOCKS, a.last - a.first));
-            a.partial0 = done;
-            done += blocks;
-            a.partials = l == launches - 1 ? done : 0;
+            a.partial = o->partials + partials;
+            partials += blocks;
             hipLaunchKernelGGL(adamw_norm_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, s, a);
         }
     }
     AdamwArgs a{};
     a.tensors = o->tensors; a.chunks = (const int2*)o->chunks; a.ctl = (AdamwControl*)o->control; a.clip = clip;
+    a.partial = o->partials; a.partials = partials; a.max_norm = max_norm;
     a.m = o->m; a.v = o->v; a.m_scale = o->m_scale; a.r_scale = o->r_scale;
     a.lr = lr; a.lr_ptr = lr_ptr; a.b1 = o->beta1; a.b2 = o->beta2; a.eps = o->eps; a.grad_scale = grad_scale; a.seed = o->seed;
     for (int l = 0; l < launches; ++l) {

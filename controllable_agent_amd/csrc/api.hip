@@ -1416,8 +1416,8 @@ static void i8_carve(int M, int K, size_t* scale_at, size_t* rest_at) {
     *rest_at = *scale_at + ((size_t)M * 4 + 15) / 16 * 16;
 }
 
-size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K) {
-    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K) return 0;
+size_t fbhip_linear_i8_workspace(const void* x, int64_t ldx, int32_t x_type, int32_t M, int32_t N, int32_t K) {
+    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K || linear_i8_fused(x, ldx, x_type, M, K)) return 0;
     size_t scale_at, rest_at;
     i8_carve(M, K, &scale_at, &rest_at);
     return rest_at + fbhip_gemm_i8_workspace(M, N, K);

@@ -476,7 +476,7 @@ int fbhip_inverse(const float* A, int32_t lda, int32_t d, float scale, float* ou
 enum { FBHIP_F32 = 0, FBHIP_BF16 = 1, FBHIP_F16 = 2 };
 #define FBHIP_GRAD_DENSE 4                 /* gradient type flag: the gradient of a row-strided parameter is itself dense */
 #define FBHIP_ADAMW_CHUNK 2048             /* elements of a tensor that one workgroup takes at a time */
-#define FBHIP_ADAMW_CONTROL_BYTES 64
+#define FBHIP_ADAMW_CONTROL_BYTES 2304
 /* One parameter, in DEVICE memory.  cols == 0: one dense run of numel elements (in storage order); cols > 0: a row-major matrix of
  * numel / cols rows with leading dimension ld >= cols.  at: its first element in the moment arrays, a multiple of 256. */
 typedef struct fbhip_adamw_tensor {
@@ -530,7 +530,7 @@ size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K);
 int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                   int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);
 /* The same with x quantised row by row on the way (fbhip_quantize_rows into the workspace). */
-size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K);
+size_t fbhip_linear_i8_workspace(const void* x, int64_t ldx, int32_t x_type, int32_t M, int32_t N, int32_t K);      /* 0: one launch does both */
 int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                     int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);
 
