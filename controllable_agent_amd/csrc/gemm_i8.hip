@@ -225,6 +225,7 @@ __device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int 
         int* o = p.partial + ((size_t)blockIdx.y * p.M + m) * ldp + n;
         const int c = lane % LANES * 4;
         if (c < cols)
+#pragma unroll 4
             for (int r = lane / LANES; r < rows; r += 64 / LANES) *(intx4*)(o + (size_t)r * ldp + c) = *(const intx4*)(box + r * ld + c);
         return;
     }
@@ -233,6 +234,7 @@ __device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int 
         const int c = lane % LANES * 4;
         if (c >= cols) return;
         const float4 s = *(const float4*)(sw + c), b = *(const float4*)(bias + c);
+#pragma unroll 4
         for (int r = lane / LANES; r < rows; r += 64 / LANES) {
             const intx4 v = *(const intx4*)(box + r * ld + c);
             const float t = sa[r];
@@ -244,6 +246,7 @@ __device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int 
     const int c = lane % COLS;           // one value a lane
     if (c >= cols) return;
     const float s = sw[c], b = bias[c];
+#pragma unroll 8
     for (int r = lane / COLS; r < rows; r += 64 / COLS) {
         const float y = i8_value(p, box[r * ld + c], sa[r], s, b);
         const size_t at = (size_t)(m + r) * p.ldy + n + c;
@@ -338,11 +341,11 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
         i8_load_lds(lds0 + (uint32_t)((s % S) * T::STAGE + piece * 1024), from, (piece * T::PIECE_ROWS < T::BN ? wbase : abase) + (size_t)(k_first + s) * BK);
     };
 
-    // the tile's scales and bias wait behind the tiles: at the end a lane needs 4 FN channels' and FM tokens'
+    // the tile's scales and bias wait behind the tiles: at the end a lane needs FN channels' and FM tokens'.  Their loads go first
     float *sw = (float*)(smem + T::TILES), *bias = sw + T::BN, *sa = bias + T::BN;
-    for (int c = threadIdx.x; c < T::BN; c += T::THREADS) { sw[c] = i8_channel(p.sw, n0 + c, p.N); bias[c] = i8_channel(p.bias, n0 + c, p.N); }
-    for (int c = threadIdx.x; c < T::BM; c += T::THREADS) sa[c] = i8_channel(p.sa, m0 + c, p.M);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");          // (the loop counts the loads that are under way)
+    static_assert(T::THREADS >= T::BN && T::THREADS >= T::BM, "a thread for each channel and token of the tile");
+    const float edge_sw = i8_channel(p.sw, n0 + (int)threadIdx.x, p.N), edge_bias = i8_channel(p.bias, n0 + (int)threadIdx.x, p.N);
+    const float edge_sa = i8_channel(p.sa, m0 + (int)threadIdx.x, p.M);
 
     const int l31 = lane & 31, half = lane >> 5, wn = wave % WN, wm = wave / WN;
     const int wrow = wn * FN * 32 + l31, arow = T::BN + wm * FM * 32 + l31;
@@ -366,6 +369,9 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
 #pragma unroll
             for (int q = 0; q < T::PIECES; ++q) issue(s, q);
         }
+    if ((int)threadIdx.x < T::BN) { sw[threadIdx.x] = edge_sw; bias[threadIdx.x] = edge_bias; }
+    if ((int)threadIdx.x < T::BM) sa[threadIdx.x] = edge_sa;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (steps >= S) i8_wait_loads<(S - 1) * T::PIECES>();
     else i8_wait_loads<0>();
     __builtin_amdgcn_s_barrier();
@@ -608,26 +614,33 @@ static hipError_t launch_i8_tile(I8Problem p, int slices, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr int I8_STRIP_TOKENS = 64;
-
+// Which kernel.  Measured with fp32 outputs, from codes, launches back to back in a graph (us):
+//   strips up to 32 tokens, and up to 64 where the weights take up to 32 MB: 1024 x 1024 with 64 tokens 4.8 (tile 5.9), 4096 x 4096 with 64 tokens
+//   11.8 (tile 13), 8192 x 8192 with 64 tokens 27.5 (tile 17.3); a long K with few channels is for the tiles, which can split it: 64 x 64 x 65536 140 as
+//   four strips;
+//   256 x 256 from 192 tiles on: 2500 x 5001 x 1999 (200 tiles) 42.8, 128 x 128 47.8; with 128 tiles (4096 x 2048 x 2048) 32.0 and 24.5;
+//   128 x 128 from 192 tiles on: 2048 x 2048 x 1024 (256 tiles) 11.1, 64 x 64 12.5; with 128 tiles (1024 x 2048 x 1024) 9.4 and 8.2;
+//   64 x 64 below, four steps deep while two such workgroups a CU are enough: 256 x 4096 x 4096 13.1, two steps deep 14.9; 1024 tiles
+//   (2048 x 2048 x 1024) 14.1 and 12.5.  K over several workgroups costs 4 us for the second launch and saves 0.28 us a step: from 32 steps
+//   and with CUs to spare only.
 I8Plan gemm_i8_plan(int M, int N, int K) {
     I8Plan plan{};
     const int steps = (K + I8_BK - 1) / I8_BK;
     plan.slices = 1;
     plan.steps = steps;
-    if (M <= I8_STRIP_TOKENS) { plan.tile = 16; return plan; }
+    const bool long_k = K > 16384 && N < 2048;
+    if (!long_k && (M <= 32 || (M <= 64 && (int64_t)N * K <= (int64_t)1 << 25))) { plan.tile = 16; return plan; }
     const int64_t t256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256), t128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
     const int64_t t64 = (int64_t)((M + 63) / 64) * ((N + 63) / 64);
     if (t256 >= 192) plan.tile = 256;
     else if (t128 >= 192) plan.tile = 128;
     else {
         plan.tile = 64;
-        int slices = (int)((384 + t64 - 1) / t64);
-        slices = std::max(1, std::min(slices, steps / 4));
-        plan.slices = slices;
+        if (t64 <= 128 && steps >= 32) plan.slices = (int)std::min<int64_t>(256 / t64, steps / 8);
+        plan.steps = (steps + plan.slices - 1) / plan.slices;
+        plan.slices = (steps + plan.steps - 1) / plan.steps;
+        plan.deep = t64 * plan.slices <= 512;
     }
-    plan.steps = (steps + plan.slices - 1) / plan.slices;
-    plan.slices = (steps + plan.steps - 1) / plan.steps;
     return plan;
 }
 
@@ -677,6 +690,7 @@ hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
     hipError_t e;
     if (plan.tile == 256) e = launch_i8_tile<4, 4, 2, 2, 128, 2>(p, plan.slices, s);
     else if (plan.tile == 128) e = launch_i8_tile<2, 4, 2, 1, 128, 2>(p, plan.slices, s);
+    else if (plan.deep) e = launch_i8_tile<2, 2, 1, 1, 128, 4>(p, plan.slices, s);
     else e = launch_i8_tile<2, 2, 1, 1, 128, 2>(p, plan.slices, s);
     if (e != hipSuccess || plan.slices == 1) return e;
     const int64_t quads = (int64_t)p.M * ((p.N + 3) / 4);

@@ -210,7 +210,7 @@ struct I8Problem {
     int M, N, K, ytype, relu, yvec, steps;   // steps: of 128 along K that a workgroup takes
     int64_t lda, ldw, ldy;
 };
-struct I8Plan { int tile, slices, steps; };
+struct I8Plan { int tile, slices, steps, deep; };
 I8Plan gemm_i8_plan(int M, int N, int K);
 hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s);
 bool linear_i8_fused(const void* x, int64_t ldx, int xtype, int M, int K);          // the tokens are quantised by the product's own launch
