@@ -21,7 +21,7 @@ BLOCK = 256            # elements that share a scale of an 8-bit moment
 CHUNK = 2048           # FBHIP_ADAMW_CHUNK
 GRAD_DENSE = 4         # FBHIP_GRAD_DENSE
 CONTROL_BYTES = 2304   # FBHIP_ADAMW_CONTROL_BYTES
-_SHAPE_TYPE_DEVICE = operator.attrgetter("shape", "dtype", "device")
+_DTYPE = operator.attrgetter("dtype")
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -65,8 +65,9 @@ class AdamW:
     r = sqrt(v) as e4m3 codes with a power-of-two scale for each 256 elements of a tensor, rounded at random (``seed``).
 
     State: ``m``, ``v`` (float32) or ``m8``, ``m_scale``, ``r8``, ``r_scale``, flat over all tensors, each tensor padded to a multiple of 256
-    elements; ``step_count``, kept on the device, so that a captured and replayed ``step`` counts too.  The same instance must not step on
-    two streams at once; a step belongs to the stream that is current when it is called.
+    elements; ``step_count``, kept on the device, so that a captured and replayed ``step`` counts too (numbers given to a captured step, ``lr``,
+    ``grad_scale``, ``max_norm``, stay what they were; so does the seed).  The same instance must not step on two streams at once; a step belongs
+    to the stream that is current when it is called.  A parameter whose storage is exchanged afterwards (``p.data = ...``) is not followed.
     """
 
     def __init__(self, params: tp.Iterable[torch.Tensor], lr: tp.Union[float, torch.Tensor] = 1e-3, betas: tp.Tuple[float, float] = (0.9, 0.999),
@@ -80,7 +81,11 @@ class AdamW:
             raise ValueError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and (eps == 0.0 or 1e-30 <= eps < math.inf)):
             raise ValueError(f"AdamW: 0 <= beta < 1 and eps 0 or at least 1e-30, got betas={betas}, eps={eps}")
+        if not isinstance(lr, torch.Tensor) and not math.isfinite(lr):
+            raise ValueError(f"AdamW: a finite lr expected, got {lr}")
         wd, scale = _per_tensor("weight_decay", weight_decay, n), _per_tensor("lr_scale", lr_scale, n)
+        if min(wd) < 0:
+            raise ValueError("AdamW: weight_decay >= 0 expected")
         self._layouts: tp.List[tp.Tuple[int, int]] = []          # (cols, ld); cols 0: dense
         spans = []
         for k, p in enumerate(self.params):
@@ -99,10 +104,14 @@ class AdamW:
             if p.numel():
                 spans.append((p.data_ptr(), p.data_ptr() + extent * p.element_size(), k))
         spans.sort()
-        for (a0, a1, i), (b0, _, j) in zip(spans, spans[1:]):
-            # column slices of one matrix may interleave; anything else that overlaps would be moved twice
-            if b0 < a1 and not (b0 != a0 and self._interleaved(i, j)):
-                raise ValueError(f"AdamW: parameters {i} and {j} share memory")
+        open_spans: tp.List[tp.Tuple[int, int, int]] = []
+        for start, end, j in spans:
+            open_spans = [o for o in open_spans if o[1] > start]
+            for other, _, i in open_spans:
+                # column slices of one matrix may interleave; anything else that overlaps would be moved twice
+                if other == start or not self._interleaved(i, j):
+                    raise ValueError(f"AdamW: parameters {i} and {j} share memory")
+            open_spans.append((start, end, j))
         self.device = self.params[0].device
         if self.device.type != "cuda":
             raise RuntimeError("AdamW: device tensors expected: controllable_agent_amd has no CPU fallback")
@@ -141,8 +150,8 @@ class AdamW:
                          None if state_bits == 32 else self.r_scale.data_ptr(), self._control.data_ptr(), self._partials.data_ptr(),
                          *self.betas, self.eps)
         self._opt_ref = C.byref(self._opt)
-        self._seen: tp.Any = None
-        self._seen_strides: tp.Any = None
+        self._seen: tp.Any = None                  # strides, sizes, types and devices that passed the checks, and what they gave
+        self._row_strided = any(cols for cols, _ in self._layouts)
         self._types = b""
         self._set_step(0)
 
@@ -163,11 +172,12 @@ class AdamW:
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} parameters")
         try:
-            seen = list(map(_SHAPE_TYPE_DEVICE, grads))
-            strides = list(map(torch.Tensor.stride, grads))
+            # (strides and size fix a dense tensor's shape; a row-strided matrix's is asked for)
+            seen = (list(map(torch.Tensor.stride, grads)), list(map(torch.Tensor.numel, grads)), list(map(_DTYPE, grads)),
+                    list(map(torch.Tensor.get_device, grads)), [g.shape for g in grads] if self._row_strided else None)
         except (AttributeError, TypeError):
             raise ValueError("AdamW.step: a gradient is no tensor: leave its parameter out, or pass zeros (which decay its moments)") from None
-        if seen == self._seen and strides == self._seen_strides:        # shapes, types, devices and strides as in the last step
+        if seen == self._seen:                     # as in the last step
             return self._types
         types = bytearray()
         for k, (g, p) in enumerate(zip(grads, self.params)):
@@ -183,7 +193,7 @@ class AdamW:
                                      "contiguous gradient of a row-strided matrix, expected")
                 flag = GRAD_DENSE
             types.append(_TYPES[g.dtype] | flag)
-        self._seen, self._seen_strides, self._types = seen, strides, bytes(types)
+        self._seen, self._types = seen, bytes(types)
         return self._types
 
     @torch.no_grad()
@@ -206,6 +216,8 @@ class AdamW:
             lr_ptr = lr.data_ptr()
         else:
             lr_value = float(lr)
+        if not (math.isfinite(lr_value) and math.isfinite(grad_scale)):
+            raise ValueError(f"AdamW.step: finite lr and grad_scale expected, got {lr} and {grad_scale}")
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"AdamW.step: max_norm > 0 expected, got {max_norm}")
         pointers = array.array("Q", map(torch.Tensor.data_ptr, grads))

@@ -1,7 +1,7 @@
 // Matrix product in 8-bit integers: y[m, n] = act( (sum_k a[m, k] w[n, k]) * sa[m] * sw[n] + bias[n] ), with a scale for each row of both
 // operands, and the row quantiser that makes them: s = max|x| / 127, code = nearest whole number to x / s (ties to even).
 //
-// The sum is exact: |sum| <= K 127^2 < 2^31 up to K = 131072, the largest that the entry points take, whatever the order of the additions, so K may
+// The sum is exact: |sum| <= K 128^2 < 2^31 up to K = 131071, the largest that the entry points take, whatever the order of the additions, so K may
 // be split at will.  It is turned into a float once (24 bits) and scaled in single precision.
 #include "common.h"
 #include "host.h"

@@ -244,7 +244,14 @@ def _code_rows(q: torch.Tensor, scale: torch.Tensor, name: str) -> tp.Tuple[int,
     return rows, K, ld
 
 
-def _i8_output(out, out_dtype, bias, M, N, device):
+def _bytes_of(t: torch.Tensor) -> tp.Tuple[int, int]:
+    """first and last byte (exclusive) of a matrix or vector with contiguous rows"""
+    last = (t.shape[0] - 1) * t.stride(0) + (t.shape[1] if t.dim() == 2 else 1) if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+
+
+def _i8_output(out, out_dtype, M, N, device, bias, inputs):
+    """(output, its row stride) after the checks of the bias and of a given output"""
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1) or bias.device != device):
         raise ValueError(f"bias: {N} contiguous float32 on {device} expected, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
     if out is None:
@@ -254,6 +261,11 @@ def _i8_output(out, out_dtype, bias, M, N, device):
     rows, cols, ld, _ = _float_rows(out, "out")
     if (rows, cols) != (M, N) or out.device != device:
         raise ValueError(f"out: [{M}, {N}] on {device} expected, got {tuple(out.shape)} on {out.device}")
+    first, last = _bytes_of(out)
+    for t in inputs + (() if bias is None else (bias,)):
+        a, b = _bytes_of(t)
+        if a < last and first < b:
+            raise ValueError("out: shares memory with an input")
     return out, ld
 
 
@@ -280,14 +292,14 @@ def gemm_i8(A: torch.Tensor, a_scale: torch.Tensor, B: torch.Tensor, b_scale: to
             relu: bool = False, out_dtype: torch.dtype = torch.float32, out: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
     """C[m, n] = act((sum_k A[m, k] B[n, k]) * a_scale[m] * b_scale[n] + bias[n]) on int8 codes A [M, K] (tokens) and B [N, K] (channels).
 
-    The sums are exact (K <= 131072).  Rows lie on 16-byte boundaries and can be read to a multiple of 16, as ``quantize_rows`` makes them.
+    The sums are exact (K <= 131071).  Rows lie on 16-byte boundaries and can be read to a multiple of 16, as ``quantize_rows`` makes them.
     """
     M, K, lda = _code_rows(A, a_scale, "A")
     N, K2, ldb = _code_rows(B, b_scale, "B")
     if K != K2 or A.device != B.device:
         raise ValueError(f"A {tuple(A.shape)} on {A.device} and B {tuple(B.shape)} on {B.device} do not go together")
     stream = _stream_on(A)
-    C, ldc = _i8_output(out, out_dtype, bias, M, N, A.device)
+    C, ldc = _i8_output(out, out_dtype, M, N, A.device, bias, (A, a_scale, B, b_scale))
     if M == 0 or N == 0:
         return C
     lib = _lib.load()
@@ -303,14 +315,14 @@ def linear_i8(x: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, *, bias: 
     """act(x W^T + bias) with x quantised row by row on the way: ``gemm_i8(*quantize_rows(x), W, w_scale, ...)`` in one call.
 
     x: float32, bfloat16 or float16 [M, K] with contiguous rows; W, w_scale: ``quantize_rows`` of the [N, K] weights; the output has x's type
-    unless ``out_dtype`` or ``out`` says otherwise.
+    unless ``out_dtype`` or ``out`` says otherwise.  For answers, not for training: no gradient flows through the codes.
     """
     M, K, ldx, code = _float_rows(x, "x")
     N, K2, ldw = _code_rows(W, w_scale, "W")
     if K != K2 or x.device != W.device:
         raise ValueError(f"x {tuple(x.shape)} on {x.device} and W {tuple(W.shape)} on {W.device} do not go together")
     stream = _stream_on(x)
-    y, ldy = _i8_output(out, x.dtype if out_dtype is None else out_dtype, bias, M, N, x.device)
+    y, ldy = _i8_output(out, x.dtype if out_dtype is None else out_dtype, M, N, x.device, bias, (x, W, w_scale))
     if M == 0 or N == 0:
         return y
     lib = _lib.load()

@@ -18,6 +18,9 @@ def _p(*shape, dtype=torch.float32):
     (dict(params=[_p(3)], betas=(1.0, 0.9)), ValueError),
     (dict(params=[_p(3)], betas=(0.9, -0.1)), ValueError),
     (dict(params=[_p(3)], eps=-1.0), ValueError),
+    (dict(params=[_p(3)], eps=1e-40), ValueError),
+    (dict(params=[_p(3)], lr=float("inf")), ValueError),
+    (dict(params=[_p(3)], weight_decay=-0.1), ValueError),
     (dict(params=[_p(3)], weight_decay=[0.1, 0.2]), ValueError),
     (dict(params=[_p(3)], weight_decay=float("nan")), ValueError),
     (dict(params=[_p(3), _p(2)], lr_scale=[1.0]), ValueError),
@@ -35,7 +38,8 @@ def test_constructor_refusals(kw, error):
 
 def test_parameters_that_share_memory_are_refused():
     flat = _p(100)
-    for params in ([flat, flat], [flat[:60], flat[50:]], [flat.view(10, 10)[:, :6], flat.view(10, 10)[:, 5:]], [flat.view(10, 10)[:, :6], flat]):
+    for params in ([flat, flat], [flat[:60], flat[50:]], [flat.view(10, 10)[:, :6], flat.view(10, 10)[:, 5:]], [flat.view(10, 10)[:, :6], flat],
+                   [flat.view(10, 10)[:, :5], flat.view(10, 10)[1:, 6:8], flat.view(10, 10)[2:, 3:4]]):
         with pytest.raises(ValueError, match="share memory"):
             AdamW(params)
     # column slices of one matrix do not overlap: refused for the missing device only

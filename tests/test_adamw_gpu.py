@@ -428,7 +428,8 @@ def test_refusals_on_the_device(AdamW):
                          ([torch.zeros(8, 1, device="cuda").expand(8, 6), h], ValueError)):
         with pytest.raises(error):
             opt.step(grads)
-    for kw in (dict(max_norm=0.0), dict(max_norm=math.nan), dict(lr=torch.zeros(1)), dict(lr=torch.zeros(2, device="cuda"))):
+    for kw in (dict(max_norm=0.0), dict(max_norm=math.nan), dict(lr=torch.zeros(1)), dict(lr=torch.zeros(2, device="cuda")),
+               dict(lr=math.nan), dict(grad_scale=math.inf)):
         with pytest.raises(ValueError):
             opt.step([g, h], **kw)
     with pytest.raises(ValueError):

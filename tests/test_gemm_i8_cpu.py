@@ -34,6 +34,21 @@ def test_float_matrices_that_are_refused():
             K._float_rows(x, "x")
 
 
+def test_outputs_that_are_refused():
+    buf = torch.zeros(200)
+    x, bias = buf[:60].view(3, 20), buf[100:105]
+    cpu = x.device
+    assert K._i8_output(buf[60:75].view(3, 5), None, 3, 5, cpu, bias, (x,))[1] == 5
+    for out in (buf[59:74].view(3, 5), buf[96:111].view(3, 5), torch.zeros(5, 3), torch.zeros(3, 10)[:, ::2], torch.zeros(1, 5).expand(3, 5)):
+        with pytest.raises(ValueError):
+            K._i8_output(out, None, 3, 5, cpu, bias, (x,))
+    for b in (torch.zeros(4), torch.zeros(5, dtype=torch.float64), torch.zeros(10)[::2]):
+        with pytest.raises(ValueError):
+            K._i8_output(None, torch.float32, 3, 5, cpu, b, (x,))
+    with pytest.raises(ValueError):
+        K._i8_output(None, torch.int8, 3, 5, cpu, None, (x,))
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros(4, 20)
     q, s = _codes(4, 20), torch.ones(4)
@@ -47,20 +62,20 @@ def test_host_tensors_are_refused():
 
 def test_c_entries_refuse_bad_calls():
     lib = _lib.load()
-    ok = dict(a=16, lda=2000, sa=16, w=16, ldw=2000, sw=16, bias=None, relu=0, y=16, ldy=4, yt=0, M=400, N=4, K=2000, ws=16)
+    ok = dict(a=16, lda=20000, sa=16, w=16, ldw=20000, sw=16, bias=None, relu=0, y=16, ldy=4, yt=0, M=400, N=4, K=20000, ws=16)
 
     def gemm(**kw):
         d = dict(ok, **kw)
         return lib.fbhip_gemm_i8(d["a"], d["lda"], d["sa"], d["w"], d["ldw"], d["sw"], d["bias"], d["relu"], d["y"], d["ldy"], d["yt"], d["M"], d["N"],
                                  d["K"], d["ws"], None)
-    for kw in (dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(y=None), dict(M=0), dict(N=0), dict(K=0), dict(K=131073, lda=131088, ldw=131088),
-               dict(a=8), dict(w=8), dict(lda=2004), dict(ldw=2004), dict(lda=1984), dict(ldw=1984), dict(ldy=3), dict(ws=None), dict(ws=8), dict(yt=3), dict(yt=-1),
+    for kw in (dict(a=None), dict(sa=None), dict(w=None), dict(sw=None), dict(y=None), dict(M=0), dict(N=0), dict(K=0), dict(K=131072, lda=131072, ldw=131072),
+               dict(a=8), dict(w=8), dict(lda=20004), dict(ldw=20004), dict(lda=19984), dict(ldw=19984), dict(ldy=3), dict(ws=None), dict(ws=8), dict(yt=3), dict(yt=-1),
                dict(ldw=1 << 24), dict(lda=1 << 24), dict(M=2 ** 31 - 1, N=2 ** 31 - 1, ldy=2 ** 31)):
         assert gemm(**kw) == -1 and lib.fbhip_last_error(None), kw
-    def lin(x=16, ldx=2000, xt=0, ws=16, **kw):
+    def lin(x=16, ldx=20000, xt=0, ws=16, **kw):
         d = dict(ok, **kw)
         return lib.fbhip_linear_i8(x, ldx, xt, d["w"], d["ldw"], d["sw"], None, 0, d["y"], d["ldy"], d["yt"], d["M"], d["N"], d["K"], ws, None)
-    assert all(r == -1 for r in (lin(x=None), lin(ldx=1999), lin(xt=3), lin(ws=None), lin(ws=8), lin(w=None), lin(K=0)))
+    assert all(r == -1 for r in (lin(x=None), lin(ldx=19999), lin(xt=3), lin(ws=None), lin(ws=8), lin(w=None), lin(K=0)))
 
     def quant(x=16, ldx=20, xt=0, q=16, ldq=32, s=16, rows=4, k=20, kp=32):
         return lib.fbhip_quantize_rows(x, ldx, xt, q, ldq, s, rows, k, kp, None)

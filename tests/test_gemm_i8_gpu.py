@@ -68,16 +68,17 @@ def test_epilogue(K, M, N, Kd, with_bias, relu, dtype):
     _check(K.gemm_i8(a, sa, w, sw, bias=bias, relu=relu, out_dtype=dtype), a, sa, w, sw, bias, relu, dtype)
 
 
-@pytest.mark.parametrize("M,N,Kd", [(1, 40, 131072), (40, 24, 131072), (300, 200, 16384)])
-def test_largest_sums(K, M, N, Kd):
-    """all codes 127: the sums reach 127^2 K = 2.1e9 < 2^31 at the largest K"""
-    a = torch.full((M, Kd), 127, dtype=torch.int8, device="cuda")
-    w = torch.full((N, Kd), 127, dtype=torch.int8, device="cuda")
-    w[1::2] = -127
+@pytest.mark.parametrize("M,N,Kd", [(1, 40, 131071), (40, 24, 131071), (1, 2100, 131071), (300, 200, 16384)])
+@pytest.mark.parametrize("code", [127, -128])
+def test_largest_sums(K, M, N, Kd, code):
+    """all codes of the largest magnitude: the sums reach 128^2 K = 2^31 - 16384 at the largest K"""
+    full = lambda r: torch.full((r, (Kd + 15) // 16 * 16), code, dtype=torch.int8, device="cuda")[:, :Kd]  # noqa: E731
+    a, w = full(M), full(N)
+    w[1::2] = 127
     one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
     y = K.gemm_i8(a, one(M), w, one(N)).double()
-    want = 127.0 * 127.0 * Kd
-    assert ((y[:, 0::2] - want).abs() <= E * want).all() and ((y[:, 1::2] + want).abs() <= E * want).all()
+    even, odd = float(code * code * Kd), float(code * 127 * Kd)
+    assert ((y[:, 0::2] - even).abs() <= E * abs(even)).all() and ((y[:, 1::2] - odd).abs() <= E * abs(odd)).all()
 
 
 @pytest.mark.parametrize("M,N,Kd", [(1, 37, 100), (7, 37, 100), (100, 37, 100), (700, 600, 100)])
@@ -207,11 +208,11 @@ def test_refusals_on_the_device(K):
     for call in (lambda: K.linear_i8(x, v, t), lambda: K.gemm_i8(w, s, v, t), lambda: K.linear_i8(x, w, s, bias=torch.zeros(5, device="cuda")),
                  lambda: K.linear_i8(x, w, s, bias=torch.zeros(6)), lambda: K.linear_i8(x, w, s, out=torch.zeros(4, 5, device="cuda")),
                  lambda: K.linear_i8(x, w, s, out_dtype=torch.float64), lambda: K.linear_i8(x, w, s, out=torch.zeros(6, 4, device="cuda").t()),
-                 lambda: K.linear_i8(x.cpu(), w, s), lambda: K.linear_i8(x, w, s, out=torch.zeros(1, 6, device="cuda").expand(4, 6))):
+                 lambda: K.linear_i8(x.cpu(), w, s), lambda: K.linear_i8(x, w[:, :20], s, out=x[:, :6]), lambda: K.linear_i8(x, w, s, out=torch.zeros(1, 6, device="cuda").expand(4, 6))):
         with pytest.raises(ValueError):
             call()
     with pytest.raises(RuntimeError, match="FBHIP_I8_MAX_K"):
-        z = torch.zeros(1, 131088, dtype=torch.int8, device="cuda")
+        z = torch.zeros(1, 131072, dtype=torch.int8, device="cuda")
         K.gemm_i8(z, torch.ones(1, device="cuda"), z, torch.ones(1, device="cuda"))
 
 
