@@ -196,7 +196,6 @@ class AdamW:
         self._seen, self._types = seen, bytes(types)
         return self._types
 
-    @torch.no_grad()
     def step(self, grads: tp.Sequence[torch.Tensor], *, lr: tp.Union[float, torch.Tensor, None] = None, grad_scale: float = 1.0,
              max_norm: tp.Optional[float] = None) -> tp.Optional[torch.Tensor]:
         """One step with the gradients ``grads`` (one for each parameter, its shape and strides; float32, bfloat16 or float16), times ``grad_scale``.
@@ -224,7 +223,7 @@ class AdamW:
         args = (self._opt_ref, pointers.buffer_info()[0], types, lr_ptr, lr_value, float(grad_scale), int(max_norm is not None),
                 0.0 if max_norm is None else float(max_norm))
         if torch.cuda.current_device() == self.device.index:
-            check(_lib.load().fbhip_adamw_step(*args, torch.cuda.current_stream().cuda_stream))
+            check(_lib.load().fbhip_adamw_step(*args, torch._C._cuda_getCurrentRawStream(self.device.index)))
         else:
             with torch.cuda.device(self.device):
                 check(_lib.load().fbhip_adamw_step(*args, torch.cuda.current_stream().cuda_stream))
