@@ -11,17 +11,12 @@ using namespace fbhip;
 using namespace fbhip::host;
 
 // ---- launching graphs with parallel branches ----------------------------------------------------------------------------
-// hipGraphLaunch of an exec whose graph has n > 1 branches can walk off the end of the exec's parallel-stream list and crash
-// the process (ROCm 7.0's libamdhip64 as bundled with torch 2.10: hip::Graph::UpdateStreams).  At instantiate time the runtime
-// creates n extra NORMAL-priority streams; at every launch it hands them to the branches, SKIPPING each extra stream that shares
-// its hardware queue with the launch stream -- without a bound on the index.  One such collision is provided for; two (both
-// extra streams of a two-branch graph on the launch stream's queue) are not.  Streams take the least-used of the 4 hardware
-// queues of their priority class, so it depends on the process's history of stream creations / destructions: a process that
-// builds and drops many contexts hit it in 3 of 6 suite runs in round 2, one in five in round 3 (backtrace:
-// profiles/r03_segv_backtrace.txt); tools/graph_queue_collision.hip reproduces it in ~40 trials of random stream churn.
-// The hardware queue of a HIGH-priority stream comes from another pool and can never be shared with those extra streams (same
-// tool: 3000 of 3000 trials): graphs with parallel branches are therefore launched from a high-priority stream of the
-// library's own, ordered behind and ahead of the caller's stream with two events (no host synchronisation).
+// On ROCm 7.0 as bundled with torch 2.10, hipGraphLaunch of a graph with parallel branches can end the process with a segmentation
+// fault (backtrace: profiles/r03_segv_backtrace.txt).  It depends on the process's history of stream creations and destructions: a
+// process that builds and drops many contexts met it in about one suite run in three.  Seen only with a launch stream of NORMAL
+// priority; from a high-priority stream 3000 of 3000 trials of random stream churn came through (profiles/r03_graph_queue_collision.txt).
+// Graphs with parallel branches are therefore launched from a high-priority stream of the library's own, ordered behind and ahead of
+// the caller's stream with two events (no host synchronisation).
 namespace {
 
 constexpr int MAX_DEVICES = 64;
@@ -46,14 +41,10 @@ hipError_t launch_stream(hipStream_t* out) {
     return hipSuccess;
 }
 
-// May this process replay graphs with parallel branches at all?  The guard above rests on two properties of the HIP runtime that no
-// public API exposes (hardware-queue identity is runtime-internal: tools/stream_queue_probe.hip reads it through object offsets of
-// one libamdhip64 build, which a product must not do): (1) a high-priority stream's hardware queue never coincides with the
-// queues of the normal-priority streams an exec creates -- verified for the HIP 7.0 runtime torch 2.10 bundles
-// (tools/graph_queue_collision.hip: 3000 of 3000 trials) --, or (2) the runtime does not have the unbounded skip loop at all --
-// verified for HIP 7.2.  So: branched graphs on HIP 7.0.x (with the guard) and on HIP >= 7.2, provided the device has a
-// high-priority class; on any other runtime the library REFUSES them and builds its n-step graphs single-queue (the plain form:
-// same kernels and results, 3-6 % slower) instead of silently running the configuration that crashed.  FBHIP_BRANCHED_GRAPHS=1
+// May this process replay graphs with parallel branches at all?  The guard above is verified by runs, for the HIP 7.0 runtime that torch
+// 2.10 bundles; HIP 7.2 came through without it.  So: branched graphs on HIP 7.0.x (with the guard) and on HIP >= 7.2, provided the
+// device has a high-priority class; on any other runtime the library REFUSES them and builds its n-step graphs single-queue (the plain
+// form: same kernels and results, 3-6 % slower) instead of silently running the configuration that crashed.  FBHIP_BRANCHED_GRAPHS=1
 // forces them on an unlisted runtime, =0 refuses them everywhere (read at every call: tests force the fallback with it).
 const char* branched_graphs_verdict(bool* ok) {
     static const char* cached = nullptr;
@@ -65,7 +56,7 @@ const char* branched_graphs_verdict(bool* ok) {
         if (hipDeviceGetStreamPriorityRange(&lo, &hi) != hipSuccess || hi >= lo) { (void)hipGetLastError(); cached = "refused: the device has no high-priority stream class"; return; }
         const int major = v / 10000000, minor = (v / 100000) % 100;
         if (major == 7 && minor == 0) { cached_ok = true; cached = "allowed: HIP 7.0 runtime, launched from a high-priority stream (verified workaround)"; }
-        else if (major > 7 || (major == 7 && minor >= 2)) { cached_ok = true; cached = "allowed: HIP >= 7.2 runtime (no unbounded skip in hip::Graph::UpdateStreams)"; }
+        else if (major > 7 || (major == 7 && minor >= 2)) { cached_ok = true; cached = "allowed: HIP >= 7.2 runtime"; }
         else cached = "refused: unverified HIP runtime version for graphs with parallel branches (FBHIP_BRANCHED_GRAPHS=1 forces them)";
     });
     const char* e = getenv("FBHIP_BRANCHED_GRAPHS");
