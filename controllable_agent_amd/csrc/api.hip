@@ -1396,7 +1396,7 @@ int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8
     fbhip_ctx* none = nullptr;
     RC(check_i8("fbhip_gemm_i8", a, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, fbhip_gemm_i8_workspace(M, N, K)));
     if (!a_scale || ((uintptr_t)a & 15) || (lda & 15) || lda < K || lda > (int64_t)1 << 23) { g_err = "fbhip_gemm_i8: code rows on 16-byte boundaries, K <= lda <= 2^23, and their scales expected"; return FBHIP_E_INVALID; }
-    I8Problem p{a, w, a_scale, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, lda, ldw, ldy};
+    I8Problem p{a, w, a_scale, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, lda, ldw, ldy};
     HIPCK(none, launch_gemm_i8(p, (int*)workspace, (hipStream_t)stream));
     return FBHIP_OK;
 }
@@ -1420,7 +1420,7 @@ int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w,
     RC(check_i8("fbhip_linear_i8", x, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, 0));
     if (ldx < K || x_type < FBHIP_F32 || x_type > FBHIP_F16) { g_err = "fbhip_linear_i8: ldx < K or unknown input type"; return FBHIP_E_INVALID; }
     if (linear_i8_fused(x, ldx, x_type, M, K)) {
-        I8Problem p{nullptr, w, nullptr, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, 0, ldw, ldy};
+        I8Problem p{nullptr, w, nullptr, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, ldw, ldy};
         HIPCK(none, launch_linear_i8_tokens(p, x, ldx, x_type, (hipStream_t)stream));
         return FBHIP_OK;
     }
@@ -1431,7 +1431,7 @@ int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w,
     float* scale = (float*)(codes + scale_at);
     const int Kp = i8_k_padded(K);
     HIPCK(none, launch_quantize_rows(x, ldx, x_type, codes, Kp, scale, M, K, Kp, (hipStream_t)stream));
-    I8Problem p{codes, w, scale, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, Kp, ldw, ldy};
+    I8Problem p{codes, w, scale, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, Kp, ldw, ldy};
     HIPCK(none, launch_gemm_i8(p, (int*)(codes + rest_at), (hipStream_t)stream));
     return FBHIP_OK;
 }

@@ -197,22 +197,30 @@ __device__ __forceinline__ uint32_t i8_half(float y, int type) {
 
 __device__ __forceinline__ float i8_channel(const float* v, int n, int N) { return v != nullptr ? v[min(n, N - 1)] : 0.f; }
 
-// up to four neighbouring values of a row
+// Up to four neighbouring values of a row, in one store whatever the row's alignment (gfx950's global stores need none).
 __device__ __forceinline__ void i8_store4(const I8Problem& p, size_t at, int count, const float (&y)[4]) {
     if (p.ytype == FBHIP_F32) {
         float* o = (float*)p.y + at;
-        if (p.yvec && count == 4) *(float4*)o = make_float4(y[0], y[1], y[2], y[3]);
-        else
-            for (int j = 0; j < count; ++j) o[j] = y[j];
+        const float4 v = make_float4(y[0], y[1], y[2], y[3]);
+        if (count == 4) __builtin_memcpy(o, &v, 16);
+        else {
+            o[0] = y[0];
+            if (count > 1) o[1] = y[1];
+            if (count > 2) o[2] = y[2];
+        }
         return;
     }
     uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = i8_half(y[j], p.ytype);
     uint16_t* o = (uint16_t*)p.y + at;
-    if (p.yvec && count == 4) *(uint2*)o = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-    else
-        for (int j = 0; j < count; ++j) o[j] = (uint16_t)h[j];
+    const uint2 v = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    if (count == 4) __builtin_memcpy(o, &v, 8);
+    else {
+        o[0] = (uint16_t)h[0];
+        if (count > 1) o[1] = (uint16_t)h[1];
+        if (count > 2) o[2] = (uint16_t)h[2];
+    }
 }
 
 // `rows` tokens from m on, `cols` channels from n on (at most 32 x COLS), their sums in shared memory; the scales and the bias in shared memory too
@@ -229,29 +237,16 @@ __device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int 
             for (int r = lane / LANES; r < rows; r += 64 / LANES) *(intx4*)(o + (size_t)r * ldp + c) = *(const intx4*)(box + r * ld + c);
         return;
     }
-    if (p.yvec) {
-        constexpr int LANES = COLS / 4;
-        const int c = lane % LANES * 4;
-        if (c >= cols) return;
-        const float4 s = *(const float4*)(sw + c), b = *(const float4*)(bias + c);
-#pragma unroll 4
-        for (int r = lane / LANES; r < rows; r += 64 / LANES) {
-            const intx4 v = *(const intx4*)(box + r * ld + c);
-            const float t = sa[r];
-            const float y[4] = {i8_value(p, v[0], t, s.x, b.x), i8_value(p, v[1], t, s.y, b.y), i8_value(p, v[2], t, s.z, b.z), i8_value(p, v[3], t, s.w, b.w)};
-            i8_store4(p, (size_t)(m + r) * p.ldy + n + c, min(4, cols - c), y);
-        }
-        return;
-    }
-    const int c = lane % COLS;           // one value a lane
+    constexpr int LANES = COLS / 4;
+    const int c = lane % LANES * 4;
     if (c >= cols) return;
-    const float s = sw[c], b = bias[c];
-#pragma unroll 8
-    for (int r = lane / COLS; r < rows; r += 64 / COLS) {
-        const float y = i8_value(p, box[r * ld + c], sa[r], s, b);
-        const size_t at = (size_t)(m + r) * p.ldy + n + c;
-        if (p.ytype == FBHIP_F32) ((float*)p.y)[at] = y;
-        else ((uint16_t*)p.y)[at] = (uint16_t)i8_half(y, p.ytype);
+    const float4 s = *(const float4*)(sw + c), b = *(const float4*)(bias + c);
+#pragma unroll 4
+    for (int r = lane / LANES; r < rows; r += 64 / LANES) {
+        const intx4 v = *(const intx4*)(box + r * ld + c);
+        const float t = sa[r];
+        const float y[4] = {i8_value(p, v[0], t, s.x, b.x), i8_value(p, v[1], t, s.y, b.y), i8_value(p, v[2], t, s.z, b.z), i8_value(p, v[3], t, s.w, b.w)};
+        i8_store4(p, (size_t)(m + r) * p.ldy + n + c, min(4, cols - c), y);
     }
 }
 
@@ -644,11 +639,6 @@ I8Plan gemm_i8_plan(int M, int N, int K) {
     return plan;
 }
 
-static void i8_output(I8Problem& p) {
-    const size_t size = p.ytype == FBHIP_F32 ? 4 : 2;
-    p.yvec = ((uintptr_t)p.y % (4 * size) == 0) && p.ldy % 4 == 0;
-}
-
 template <int NT, int MT>
 static void launch_i8_strip(const I8Problem& p, hipStream_t s) {
     hipLaunchKernelGGL((gemm_i8_strip_kernel<NT, MT, 0>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(I8_STRIP_THREADS), 0, s, p,
@@ -668,7 +658,6 @@ bool linear_i8_fused(const void* x, int64_t ldx, int xtype, int M, int K) {
 }
 
 hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
-    i8_output(p);
     if (p.M == 1) launch_i8_strip_tokens<1>(p, x, ldx, xtype, s);
     else if (p.M == 2) launch_i8_strip_tokens<2>(p, x, ldx, xtype, s);
     else launch_i8_strip_tokens<4>(p, x, ldx, xtype, s);
@@ -677,7 +666,6 @@ hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int 
 
 hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
     const I8Plan plan = gemm_i8_plan(p.M, p.N, p.K);
-    i8_output(p);
     if (plan.tile == 16) {
         const bool wide = p.N >= 8192;
         if (p.M <= 16) launch_i8_strip<1, 1>(p, s);

@@ -207,7 +207,7 @@ struct I8Problem {
     const float *sa, *sw, *bias;
     void* y;
     int* partial;                            // [slices][M][N] where K is split
-    int M, N, K, ytype, relu, yvec, steps;   // steps: of 128 along K that a workgroup takes
+    int M, N, K, ytype, relu, steps;         // steps: of 128 along K that a workgroup takes
     int64_t lda, ldw, ldy;
 };
 struct I8Plan { int tile, slices, steps, deep; };
