@@ -10,6 +10,9 @@ namespace fbhip {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
+// four values at any address: gfx950's global stores need no alignment
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t uintx2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr int I8_BK = 128;                    // bytes of K in a step: one row of a tile is one 128-byte line
 
@@ -197,12 +200,11 @@ __device__ __forceinline__ uint32_t i8_half(float y, int type) {
 
 __device__ __forceinline__ float i8_channel(const float* v, int n, int N) { return v != nullptr ? v[min(n, N - 1)] : 0.f; }
 
-// Up to four neighbouring values of a row, in one store whatever the row's alignment (gfx950's global stores need none).
+// Up to four neighbouring values of a row, in one store whatever the row's alignment.
 __device__ __forceinline__ void i8_store4(const I8Problem& p, size_t at, int count, const float (&y)[4]) {
     if (p.ytype == FBHIP_F32) {
         float* o = (float*)p.y + at;
-        const float4 v = make_float4(y[0], y[1], y[2], y[3]);
-        if (count == 4) __builtin_memcpy(o, &v, 16);
+        if (count == 4) *(floatx4_any*)o = floatx4_any{y[0], y[1], y[2], y[3]};
         else {
             o[0] = y[0];
             if (count > 1) o[1] = y[1];
@@ -214,8 +216,7 @@ __device__ __forceinline__ void i8_store4(const I8Problem& p, size_t at, int cou
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = i8_half(y[j], p.ytype);
     uint16_t* o = (uint16_t*)p.y + at;
-    const uint2 v = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-    if (count == 4) __builtin_memcpy(o, &v, 8);
+    if (count == 4) *(uintx2_any*)o = uintx2_any{h[0] | h[1] << 16, h[2] | h[3] << 16};
     else {
         o[0] = (uint16_t)h[0];
         if (count > 1) o[1] = (uint16_t)h[1];
