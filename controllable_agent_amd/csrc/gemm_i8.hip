@@ -308,8 +308,10 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
     // workgroup b runs on XCD b % 8: each XCD takes one run of the tiles
     const int xcd = blockIdx.x & 7, each = tiles >> 3, rest = tiles & 7;
     const int t = (xcd < rest ? xcd * (each + 1) : rest * (each + 1) + (xcd - rest) * each) + ((int)blockIdx.x >> 3);
-    // ... in blocks of eight token tiles, so that its 32 CUs share 8 + 4 tiles' operands and not 1 + 32
-    const int group = t / (8 * tiles_n), g0 = group * 8, gm = min(8, tiles_m - g0), in_group = t - group * 8 * tiles_n;
+    // ... in blocks of a few token tiles, so that its 32 CUs share 4 + 8 (or 8 + 4) tiles' operands and not 1 + 32.  8192^3: 479 us with four
+    // token tiles of 256, 484 with eight; 4096 x 2048 x 2048: 24.1 with eight of 128, 24.5 with four
+    constexpr int GROUP = T::BM == 256 ? 4 : 8;
+    const int group = t / (GROUP * tiles_n), g0 = group * GROUP, gm = min(GROUP, tiles_m - g0), in_group = t - group * GROUP * tiles_n;
     const int n0 = (in_group / gm) * T::BN, m0 = (g0 + in_group % gm) * T::BM;
     const int steps_all = (p.K + BK - 1) / BK;
     const int k_first = blockIdx.y * p.steps, steps = min(p.steps, steps_all - k_first);
@@ -355,8 +357,7 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
     // The fragments of a slice are read while the slice before it is multiplied.  Before the last slice of a step everybody has read the
-    // step's tile, and the next step's has landed: step s + S goes into the place of step s, its loads spread over a step's slices (together they
-    // would fill the CU's load queue and hold up the products behind them).
+    // step's tile, and the next step's has landed: step s + S goes into the place of step s, its loads spread over a step's slices.
     const int full = steps - (tail ? 1 : 0);
     intx4 w[2][FN], a[2][FM];
 #pragma unroll
@@ -384,10 +385,8 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
             for (int j = 0; j < FM; ++j) {
                 acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[set][i], a[set][j], acc[i][j], 0, 0, 0);
                 if (done * FN * FM < (i * FM + j + 1) * count) {
-                    __builtin_amdgcn_sched_barrier(0);
                     if (live) issue(to, first + done);
                     ++done;
-                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
     };
@@ -677,7 +676,7 @@ hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
     p.steps = plan.steps;
     p.partial = plan.slices > 1 ? partial : nullptr;
     hipError_t e;
-    if (plan.tile == 256) e = launch_i8_tile<4, 4, 2, 2, 128, 2>(p, plan.slices, s);
+    if (plan.tile == 256) e = launch_i8_tile<2, 4, 4, 2, 128, 2>(p, plan.slices, s);
     else if (plan.tile == 128) e = launch_i8_tile<2, 4, 2, 1, 128, 2>(p, plan.slices, s);
     else if (plan.deep) e = launch_i8_tile<2, 2, 1, 1, 128, 4>(p, plan.slices, s);
     else e = launch_i8_tile<2, 2, 1, 1, 128, 2>(p, plan.slices, s);
