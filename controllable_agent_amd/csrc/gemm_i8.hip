@@ -1,5 +1,5 @@
 // Matrix product in 8-bit integers: y[m, n] = act( (sum_k a[m, k] w[n, k]) * sa[m] * sw[n] + bias[n] ), with a scale for each row of both
-// operands, and the row quantiser that makes them: s = max|x| / 127, code = nearest whole number to x / s (ties to even).
+// operands, and the row quantiser that makes them: s = max|x| * fl(1/127), code = nearest whole number to fl(x / s) (ties to even).
 //
 // The sum is exact: |sum| <= K 128^2 < 2^31 up to K = 131071, the largest that the entry points take, whatever the order of the additions, so K may
 // be split at will.  It is turned into a float once (24 bits) and scaled in single precision.
@@ -46,7 +46,7 @@ struct I8Row { float scale, inv; bool zero; };
 // a row that holds a NaN or an infinity: the scale NaN and codes 0; a row of zeros, or one so small that its scale is 0: codes 0
 __device__ __forceinline__ I8Row i8_row(float top, bool bad) {
     I8Row r;
-    r.scale = top / 127.f;
+    r.scale = top * (1.f / 127.f);                        // (the reciprocal rounded to float32: within a step of the quotient)
     r.zero = bad || r.scale == 0.f;
     r.inv = r.scale >= 0x1p-100f ? __builtin_amdgcn_rcpf(r.scale) : __uint_as_float(0x7FC00000u);
     if (bad) r.scale = __uint_as_float(0x7FC00000u);

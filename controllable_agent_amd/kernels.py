@@ -270,7 +270,8 @@ def _i8_output(out, out_dtype, M, N, device, bias, inputs):
 
 
 def quantize_rows(x: torch.Tensor) -> tp.Tuple[torch.Tensor, torch.Tensor]:
-    """(codes, scale): scale[r] = max|x[r]| / 127, codes = nearest whole numbers to x / scale (int8, ties to even).
+    """(codes, scale): scale[r] = max|x[r]| / 127 (as a product with the float32 nearest to 1/127), codes = nearest whole numbers to x / scale (int8,
+    ties to even).
 
     The tokens of an activation matrix and the channels of a weight matrix [out, in] alike.  x: float32, bfloat16 or float16 [rows, K] with contiguous
     rows.  ``codes`` is a view of rows padded with zeros to a multiple of 128, which ``gemm_i8`` and ``linear_i8`` read as it is.  A row that holds a NaN or an

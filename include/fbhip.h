@@ -518,7 +518,7 @@ int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, cons
 
 /* ---- matrix product in 8-bit integers (csrc/gemm_i8.hip) -------------------------------------------- */
 #define FBHIP_I8_MAX_K 131071              /* the int32 sums cannot overflow up to here: 128 * 128 * K < 2^31 */
-/* scale[r] = max|x[r, :]| / 127, codes[r, k] = nearest whole number to x[r, k] / scale[r] (ties to even).  x: FBHIP_F32 / BF16 / F16, rows
+/* scale[r] = max|x[r, :]| * (1 / 127 as a float32), codes[r, k] = nearest whole number to x[r, k] / scale[r] (ties to even).  x: FBHIP_F32 / BF16 / F16, rows
  * ldx elements apart.  codes: rows ldq bytes apart, ldq >= Kp; columns K .. Kp - 1 are set to 0.  A row with a NaN or an infinity: scale NaN,
  * codes 0; a row of zeros: scale 0, codes 0. */
 int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* codes, int64_t ldq, float* scale, int32_t rows, int32_t K,

@@ -100,10 +100,10 @@ def test_given_output_rows_and_what_lies_around_them(K, M, N, Kd, dtype):
 
 # --------------------------------------------------------------------------------------------------------------------------- quantiser
 def _want_codes(x):
-    """scale in float32, quotient rounded to float32, nearest whole number, ties to even"""
+    """scale: the product with the float32 nearest to 1/127, in float32; quotient rounded to float32, nearest whole number, ties to even"""
     x = x.cpu().float()
     top = x.abs().amax(1)
-    s = (top.double() / 127).float()
+    s = (top.double() * float(torch.tensor(1 / 127, dtype=torch.float32))).float()
     q = (x.double() / s.double().clamp_min(1e-300)[:, None]).float().round().clamp(-127, 127)
     return torch.where(s[:, None] > 0, q, torch.zeros_like(q)).to(torch.int8), s
 
