@@ -65,8 +65,8 @@ class AdamW:
     r = sqrt(v) as e4m3 codes with a power-of-two scale for each 256 elements of a tensor, rounded at random (``seed``).
 
     State: ``m``, ``v`` (float32) or ``m8``, ``m_scale``, ``r8``, ``r_scale``, flat over all tensors, each tensor padded to a multiple of 256
-    elements; ``step_count``, kept on the device, so that a captured and replayed ``step`` counts too (numbers given to a captured step, ``lr``,
-    ``grad_scale``, ``max_norm``, stay what they were; so does the seed).  The same instance must not step on two streams at once; a step belongs
+    elements; ``step_count``, kept on the device, so that a captured and replayed ``step`` counts too (it reads the gradient tensors that it was captured
+    with; the numbers given to it, ``lr``, ``grad_scale``, ``max_norm``, and the seed stay what they were).  The same instance must not step on two streams at once; a step belongs
     to the stream that is current when it is called.  A parameter whose storage is exchanged afterwards (``p.data = ...``) is not followed.
     """
 
@@ -150,6 +150,7 @@ class AdamW:
                          None if state_bits == 32 else self.r_scale.data_ptr(), self._control.data_ptr(), self._partials.data_ptr(),
                          *self.betas, self.eps)
         self._opt_ref = C.byref(self._opt)
+        self._versioned = [p for p in self.params if not p.is_inference()]       # (tensors made in inference mode have no version)
         self._seen: tp.Any = None                  # strides, sizes, types and devices that passed the checks, and what they gave
         self._row_strided = any(cols for cols, _ in self._layouts)
         self._types = b""
@@ -227,7 +228,7 @@ class AdamW:
         else:
             with torch.cuda.device(self.device):
                 check(_lib.load().fbhip_adamw_step(*args, torch.cuda.current_stream().cuda_stream))
-        torch.autograd.graph.increment_version(self.params)
+        torch.autograd.graph.increment_version(self._versioned)
         return None if max_norm is None else self._norm
 
     @property

@@ -184,7 +184,7 @@ hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q,
 
 // ------------------------------------------------------------------------------------------------------------------ epilogue
 __device__ __forceinline__ float i8_value(const I8Problem& p, int acc, float sa, float sw, float bias) {
-    const float y = (float)acc * sa * sw + bias;
+    const float y = (float)acc * (sa * sw) + bias;          // (the scales first: their product leaves the range only where the value does)
     return p.relu && y < 0.f ? 0.f : y;          // (NaN stays)
 }
 
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
         i8_load_lds(lds0 + (uint32_t)((s % S) * T::STAGE + piece * 1024), from, (piece * T::PIECE_ROWS < T::BN ? wbase : abase) + (size_t)(k_first + s) * BK);
     };
 
-    // the tile's scales and bias wait behind the tiles: at the end a lane needs FN channels' and FM tokens'.  Their loads go first
+    // the tile's scales and bias: their loads go first; at the end they lie behind the tiles, where a lane finds its 4 FN channels' and FM tokens'
     float *sw = (float*)(smem + T::TILES), *bias = sw + T::BN, *sa = bias + T::BN;
     static_assert(T::THREADS >= T::BN && T::THREADS >= T::BM, "a thread for each channel and token of the tile");
     const float edge_sw = i8_channel(p.sw, n0 + (int)threadIdx.x, p.N), edge_bias = i8_channel(p.bias, n0 + (int)threadIdx.x, p.N);
@@ -369,9 +369,6 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
 #pragma unroll
             for (int q = 0; q < T::PIECES; ++q) issue(s, q);
         }
-    if ((int)threadIdx.x < T::BN) { sw[threadIdx.x] = edge_sw; bias[threadIdx.x] = edge_bias; }
-    if ((int)threadIdx.x < T::BM) sa[threadIdx.x] = edge_sa;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (steps >= S) i8_wait_loads<(S - 1) * T::PIECES>();
     else i8_wait_loads<0>();
     __builtin_amdgcn_s_barrier();
@@ -420,6 +417,9 @@ __global__ void __launch_bounds__((I8Tile<WN, WM, FN, FM, BK, S>::THREADS), (FN 
     }
     // A wave's 32 tokens at a time go through its own part of shared memory, so that its stores are whole lines of a token's row, whatever the
     // row's alignment: a lane's accumulators lie 32 tokens apart.
+    if ((int)threadIdx.x < T::BN) { sw[threadIdx.x] = edge_sw; bias[threadIdx.x] = edge_bias; }
+    if ((int)threadIdx.x < T::BM) sa[threadIdx.x] = edge_sa;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     int* box = (int*)(smem + wave * T::BOX);
@@ -614,8 +614,8 @@ static hipError_t launch_i8_tile(I8Problem p, int slices, hipStream_t s) {
 }
 
 // Which kernel.  Measured with fp32 outputs, from codes, launches back to back in a graph (us):
-//   strips up to 32 tokens, and up to 64 where the weights take up to 32 MB: 1024 x 1024 with 64 tokens 4.8 (tile 5.9), 4096 x 4096 with 64 tokens
-//   11.8 (tile 13), 8192 x 8192 with 64 tokens 27.5 (tile 17.3); a long K with few channels is for the tiles, which can split it: 64 x 64 x 65536 140 as
+//   strips up to 16 tokens, and up to 64 where the weights take up to 32 MB: 1024 x 1024 with 64 tokens 4.6 (tile 6.3), 4096 x 4096 with 64 tokens
+//   11.9 (tile 13), 8192 x 8192 with 32 tokens 21.4 (tile 16.6); a long K with few channels is for the tiles, which can split it: 64 x 64 x 65536 140 as
 //   four strips;
 //   256 x 256 from 192 tiles on: 2500 x 5001 x 1999 (200 tiles) 42.8, 128 x 128 47.8; with 128 tiles (4096 x 2048 x 2048) 32.0 and 24.5;
 //   128 x 128 from 192 tiles on: 2048 x 2048 x 1024 (256 tiles) 11.1, 64 x 64 12.5; with 128 tiles (1024 x 2048 x 1024) 9.4 and 8.2;
@@ -628,7 +628,7 @@ I8Plan gemm_i8_plan(int M, int N, int K) {
     plan.slices = 1;
     plan.steps = steps;
     const bool long_k = K > 16384 && N < 2048;
-    if (!long_k && (M <= 32 || (M <= 64 && (int64_t)N * K <= (int64_t)1 << 25))) { plan.tile = 16; return plan; }
+    if (!long_k && (M <= 16 || (M <= 64 && (int64_t)N * K <= (int64_t)1 << 25))) { plan.tile = 16; return plan; }
     const int64_t t256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256), t128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
     const int64_t t64 = (int64_t)((M + 63) / 64) * ((N + 63) / 64);
     if (t256 >= 192) plan.tile = 256;

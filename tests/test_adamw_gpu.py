@@ -419,6 +419,17 @@ def test_autograd_sees_the_change(AdamW):
         y.backward()
 
 
+def test_in_inference_mode(AdamW):
+    gen = torch.Generator().manual_seed(15)
+    p = _randn(gen, 1000)
+    q, g = p.clone(), _randn(gen, 1000)
+    AdamW([p], lr=1e-2).step([g])
+    with torch.inference_mode():
+        r = q.clone()
+        AdamW([r], lr=1e-2).step([g.clone()])
+    assert torch.equal(p, r)
+
+
 def test_refusals_on_the_device(AdamW):
     p, q = torch.zeros(8, 6, device="cuda"), torch.zeros(5, device="cuda")
     opt = AdamW([p, q])

@@ -68,6 +68,17 @@ def test_epilogue(K, M, N, Kd, with_bias, relu, dtype):
     _check(K.gemm_i8(a, sa, w, sw, bias=bias, relu=relu, out_dtype=dtype), a, sa, w, sw, bias, relu, dtype)
 
 
+def test_scales_of_opposite_sizes(K):
+    """the product of the scales is in range where neither scale times the sum would be"""
+    gen = torch.Generator().manual_seed(9)
+    for M in (3, 40, 300):
+        a, w = _codes(gen, M, 500), _codes(gen, 70, 500)
+        sa, sw = torch.full((M,), 1e36, device="cuda"), torch.full((70,), 1e-32, device="cuda")
+        _check(K.gemm_i8(a, sa, w, sw), a, sa, w, sw, None, False, torch.float32)
+        _check(K.gemm_i8(a, sw[:1].expand(M).contiguous(), w, sa[:1].expand(70).contiguous()), a, sw[:1].expand(M), w, sa[:1].expand(70), None, False,
+               torch.float32)
+
+
 @pytest.mark.parametrize("M,N,Kd", [(1, 40, 131071), (40, 24, 131071), (1, 2100, 131071), (300, 200, 16384)])
 @pytest.mark.parametrize("code", [127, -128])
 def test_largest_sums(K, M, N, Kd, code):
