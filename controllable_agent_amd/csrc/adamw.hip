@@ -28,9 +28,10 @@ namespace fbhip {
 constexpr int ADAMW_THREADS = 256, ADAMW_PER_LANE = 8, ADAMW_CHUNK = ADAMW_THREADS * ADAMW_PER_LANE;
 static_assert(ADAMW_CHUNK == FBHIP_ADAMW_CHUNK, "the caller's chunk table counts chunks of this size");
 constexpr int ADAMW_MAX_TENSORS = 384;       // gradient addresses travel in the kernel arguments (4 KB): valid in a captured graph
-// As many workgroups as 256 CUs hold at once (80 and 95 registers: six and five); they walk the chunks.  With 2048 the second lot runs on
-// CUs that are half empty: the walker networks' step 24.2 -> 22.2 us (32 bits), 20.2 -> 16.9 us (8 bits).
-constexpr int ADAMW_BLOCKS_32 = 6 * 256, ADAMW_BLOCKS_8 = 5 * 256;
+// Workgroups that are all on the 256 CUs at once and walk the chunks (2048 of them: the second lot runs on CUs that are half empty, 24.2 and 20.2 us
+// for the walker networks).  With 32-bit moments three a CU keep memory busy, and more of them only spread the accesses: 67 M in bf16 327 us
+// with three, 330 with four, 333 with five.  With 8-bit moments the arithmetic wants all five that the registers allow: 134 M 381 us, 395 with four.
+constexpr int ADAMW_BLOCKS_32 = 3 * 256, ADAMW_BLOCKS_8 = 5 * 256;
 constexpr int ADAMW_NORM_BLOCKS = 1024;      // one partial sum each, folded in order
 
 // Workgroups count themselves off in 32 groups: 2048 additions to one address take 20 us, in turn, at the end of a step that takes 40.
@@ -97,15 +98,17 @@ __device__ __forceinline__ float load_one(const void* base, int64_t i, int type)
     return type == FBHIP_BF16 ? bf16_float(h) : fp16_float(h);
 }
 
-// eight consecutive elements from a 16-byte aligned address
+// values side by side at any address: gfx950's global loads and stores need no alignment
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t uintx4_any __attribute__((ext_vector_type(4), aligned(2)));
+
 __device__ __forceinline__ void load_eight(const void* base, int64_t i, int type, float (&x)[8]) {
     if (type == FBHIP_F32) {
-        const float4 a = *(const float4*)((const float*)base + i), b = *(const float4*)((const float*)base + i + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        const floatx4_any a = *(const floatx4_any*)((const float*)base + i), b = *(const floatx4_any*)((const float*)base + i + 4);
+        x[0] = a[0]; x[1] = a[1]; x[2] = a[2]; x[3] = a[3]; x[4] = b[0]; x[5] = b[1]; x[6] = b[2]; x[7] = b[3];
         return;
     }
-    const uint4 q = *(const uint4*)((const uint16_t*)base + i);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const uintx4_any w = *(const uintx4_any*)((const uint16_t*)base + i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         x[2 * j] = type == FBHIP_BF16 ? bf16_float(w[j] & 0xFFFFu) : fp16_float((uint16_t)w[j]);
@@ -125,7 +128,7 @@ struct Walk {
 __device__ __forceinline__ void load_grad(const fbhip_adamw_tensor& T, const void* g, int gtype, int64_t i, float (&x)[8]) {
     const bool flat = T.cols == 0 || (gtype & FBHIP_GRAD_DENSE);
     gtype &= FBHIP_GRAD_DENSE - 1;
-    if (flat && i + 8 <= T.numel && ((uintptr_t)g & 15) == 0) { load_eight(g, i, gtype, x); return; }
+    if (flat && i + 8 <= T.numel) { load_eight(g, i, gtype, x); return; }
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
     if (i >= T.numel) return;
@@ -211,7 +214,7 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a) {
+__global__ void __launch_bounds__(ADAMW_THREADS, 5) adamw_kernel(const AdamwArgs a) {
 #pragma clang fp contract(off)
     __shared__ double red[4], shared_lr, shared_ibc1;
     __shared__ float shared_rbc2, shared_gs;
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a)
         const int64_t s = T.at + i;
         float g[8], p[8], m[8], v[8];
         load_grad(T, a.grad[e.x - a.tensor0], a.gtype[e.x - a.tensor0], i, g);
-        const bool whole = T.cols == 0 && i + 8 <= T.numel && ((uintptr_t)T.p & 15) == 0;
+        const bool whole = T.cols == 0 && i + 8 <= T.numel;
         if (whole) load_eight(T.p, i, T.dtype, p);
         else {
 #pragma unroll
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a)
                 h[j] = p[j] != p[j] ? 0x7FC0u : (b + (word[j] * 0x9E3779B1u >> 16)) >> 16;
             }
             if (whole) {
-                *(uint4*)((uint16_t*)T.p + i) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                *(uintx4_any*)((uint16_t*)T.p + i) = uintx4_any{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
             } else if (i < T.numel) {
                 Walk w(i, T.cols == 0 ? 0x7FFFFFFF : T.cols, T.ld);
 #pragma unroll
@@ -336,8 +339,8 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwArgs a)
                 }
             }
         } else if (whole) {
-            *(float4*)((float*)T.p + i) = make_float4(p[0], p[1], p[2], p[3]);
-            *(float4*)((float*)T.p + i + 4) = make_float4(p[4], p[5], p[6], p[7]);
+            *(floatx4_any*)((float*)T.p + i) = floatx4_any{p[0], p[1], p[2], p[3]};
+            *(floatx4_any*)((float*)T.p + i + 4) = floatx4_any{p[4], p[5], p[6], p[7]};
         } else if (i < T.numel) {
             Walk w(i, T.cols == 0 ? 0x7FFFFFFF : T.cols, T.ld);
 #pragma unroll

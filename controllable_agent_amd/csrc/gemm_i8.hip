@@ -10,9 +10,10 @@ namespace fbhip {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
-// four values at any address: gfx950's global stores need no alignment
+// values side by side at any address: gfx950's global loads and stores need no alignment
 typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t uintx2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t uintx4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int I8_BK = 128;                    // bytes of K in a step: one row of a tile is one 128-byte line
 
@@ -70,7 +71,10 @@ __device__ __forceinline__ float i8_unpack(const uint32_t (&w)[4], int e, int ty
 template <bool WIDE>
 __device__ __forceinline__ uint4 i8_piece(const char* base, int k, int K) {
     constexpr int V = WIDE ? 4 : 8;
-    if (k + V <= K) return *(const uint4*)(base + (size_t)k * (16 / V));
+    if (k + V <= K) {
+        const uintx4_any w = *(const uintx4_any*)(base + (size_t)k * (16 / V));
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
     uint32_t w[4] = {0u, 0u, 0u, 0u};
     for (int e = 0; e < K - k; ++e) {
         if (WIDE) w[e] = ((const uint32_t*)base)[k + e];
@@ -80,8 +84,7 @@ __device__ __forceinline__ uint4 i8_piece(const char* base, int k, int K) {
 }
 
 // Bound by memory: x is read once, the codes are written once (8192^2 bf16: 35 us, 5.8 TB/s, part of it from the Infinity Cache).
-// A row in the registers of TPR threads: C pieces of 16 bytes a thread, read once.  Rows on 16-byte boundaries, K in whole pieces or not.
-// (One thread row of 64 takes up to 8 pieces: 2048 fp32 or 4096 16-bit values; a workgroup of 256 four times that.)
+// A row in the registers of TPR threads: C pieces of 16 bytes a thread, read once, whatever the row's alignment.
 template <int TPR, int C, bool WIDE>
 __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
                                                                 float* __restrict__ scale, int rows, int K, int Kp) {
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __re
     if (t == 0) scale[row] = r.scale;
 }
 
-// Any row: a workgroup reads it twice.
+// Longer rows: a workgroup reads them twice.
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
                                                             float* __restrict__ scale, int K, int Kp) {
     __shared__ float red[4];
@@ -169,15 +172,14 @@ static void launch_quantize_reg(const void* x, int64_t ldx, int type, int8_t* q,
 }
 
 hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s) {
-    const int V = type == FBHIP_F32 ? 4 : 8, size = 16 / V;
-    const bool aligned = ((uintptr_t)x & 15) == 0 && (ldx * size) % 16 == 0 && ((uintptr_t)q & 7) == 0 && ldq % 8 == 0 && Kp % 8 == 0;
-    const int pieces = (Kp + V - 1) / V;
+    const int V = type == FBHIP_F32 ? 4 : 8, pieces = (Kp + V - 1) / V;
+    const bool even = ((uintptr_t)q & 7) == 0 && ldq % 8 == 0 && Kp % 8 == 0;          // the codes' rows take whole pieces
     // a wave for a row while a row fits, unless the rows are so few that more threads a row fill the CUs sooner
-    if (aligned && pieces <= 64 * 2) launch_quantize_reg<64, 2>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
-    else if (aligned && pieces <= 64 * 4 && rows >= 2048) launch_quantize_reg<64, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
-    else if (aligned && pieces <= 256) launch_quantize_reg<256, 1>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
-    else if (aligned && pieces <= 256 * 4) launch_quantize_reg<256, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
-    else if (aligned && pieces <= 256 * 8) launch_quantize_reg<256, 8>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    if (even && pieces <= 64 * 2) launch_quantize_reg<64, 2>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (even && pieces <= 64 * 4 && rows >= 2048) launch_quantize_reg<64, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (even && pieces <= 256) launch_quantize_reg<256, 1>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (even && pieces <= 256 * 4) launch_quantize_reg<256, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
+    else if (even && pieces <= 256 * 8) launch_quantize_reg<256, 8>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
     else hipLaunchKernelGGL(quantize_rows_kernel, dim3(rows), dim3(256), 0, s, x, ldx, type, q, ldq, scale, K, Kp);
     return hipGetLastError();
 }
@@ -655,10 +657,10 @@ static void launch_i8_strip_tokens(const I8Problem& p, const void* x, int64_t ld
     hipLaunchKernelGGL((gemm_i8_strip_kernel<1, 1, TOKENS>), dim3((p.N + 15) / 16), dim3(I8_STRIP_THREADS), lds, s, p, x, ldx, xtype);
 }
 
-// Up to four tokens whose values fit four pieces of 16 bytes a thread, on 16-byte rows.
-bool linear_i8_fused(const void* x, int64_t ldx, int xtype, int M, int K) {
+// Up to four tokens whose values fit four pieces of 16 bytes a thread.
+bool linear_i8_fused(int xtype, int M, int K) {
     const int V = xtype == FBHIP_F32 ? 4 : 8, rows = M == 3 ? 4 : M;
-    return M <= 4 && ((uintptr_t)x & 15) == 0 && (M == 1 || (ldx * (16 / V)) % 16 == 0) && (K + 127) / 128 * 128 <= I8_STRIP_THREADS / rows * V * I8_STRIP_PIECES;
+    return M <= 4 && (K + 127) / 128 * 128 <= I8_STRIP_THREADS / rows * V * I8_STRIP_PIECES;
 }
 
 hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int xtype, hipStream_t s) {

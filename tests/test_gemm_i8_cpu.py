@@ -81,5 +81,6 @@ def test_c_entries_refuse_bad_calls():
         return lib.fbhip_quantize_rows(x, ldx, xt, q, ldq, s, rows, k, kp, None)
     assert all(r == -1 for r in (quant(x=None), quant(q=None), quant(s=None), quant(rows=0), quant(k=0), quant(kp=19), quant(ldq=31), quant(ldx=19),
                                  quant(xt=5)))
-    assert lib.fbhip_linear_i8_workspace(16, 20, 0, 40, 4, 20) >= 40 * 128 + 160 and lib.fbhip_linear_i8_workspace(16, 20, 0, 0, 4, 20) == 0
-    assert lib.fbhip_linear_i8_workspace(16, 20, 0, 4, 4, 20) == 0 and lib.fbhip_linear_i8_workspace(20, 20, 0, 4, 4, 20) > 0      # one launch; rows off 16 bytes
+    assert lib.fbhip_linear_i8_workspace(0, 40, 4, 20) >= 40 * 128 + 160 and lib.fbhip_linear_i8_workspace(0, 0, 4, 20) == 0
+    # up to four tokens of a row that fits: one launch, which needs none
+    assert lib.fbhip_linear_i8_workspace(0, 4, 4, 20) == 0 and lib.fbhip_linear_i8_workspace(0, 4, 4, 20000) > 0
