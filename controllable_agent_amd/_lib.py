@@ -131,7 +131,7 @@ PROTOTYPES = {
     "fbhip_quantize_rows": (C.c_int, [_P, _L, _I, _P, _L, _P, _I, _I, _I, _P]),
     "fbhip_gemm_i8_workspace": (_Z, [_I, _I, _I]),
     "fbhip_gemm_i8": (C.c_int, [_P, _L, _P, _P, _L, _P, _P, _I, _P, _L, _I, _I, _I, _I, _P, _P]),
-    "fbhip_linear_i8_workspace": (_Z, [_I, _I, _I, _I]),
+    "fbhip_linear_i8_workspace": (_Z, [_I, _I, _I]),
     "fbhip_linear_i8": (C.c_int, [_P, _L, _I, _P, _L, _P, _P, _I, _P, _L, _I, _I, _I, _I, _P, _P]),
     "fbhip_adamw_step": (C.c_int, [_P, _P, _P, _P, C.c_double, _F, _I, _F, _P]),
 }

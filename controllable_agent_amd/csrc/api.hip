@@ -1407,8 +1407,8 @@ static void i8_carve(int M, int K, size_t* scale_at, size_t* rest_at) {
     *rest_at = *scale_at + ((size_t)M * 4 + 15) / 16 * 16;
 }
 
-size_t fbhip_linear_i8_workspace(int32_t x_type, int32_t M, int32_t N, int32_t K) {
-    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K || linear_i8_fused(x_type, M, K)) return 0;
+size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K) {
+    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K || linear_i8_fused(M, K)) return 0;
     size_t scale_at, rest_at;
     i8_carve(M, K, &scale_at, &rest_at);
     return rest_at + fbhip_gemm_i8_workspace(M, N, K);
@@ -1419,7 +1419,7 @@ int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w,
     fbhip_ctx* none = nullptr;
     RC(check_i8("fbhip_linear_i8", x, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, 0));
     if (ldx < K || x_type < FBHIP_F32 || x_type > FBHIP_F16) { g_err = "fbhip_linear_i8: ldx < K or unknown input type"; return FBHIP_E_INVALID; }
-    if (linear_i8_fused(x_type, M, K)) {
+    if (linear_i8_fused(M, K)) {
         I8Problem p{nullptr, w, nullptr, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, ldw, ldy};
         HIPCK(none, launch_linear_i8_tokens(p, x, ldx, x_type, (hipStream_t)stream));
         return FBHIP_OK;

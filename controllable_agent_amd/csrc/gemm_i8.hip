@@ -464,22 +464,22 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
 // instructions' share: the operands agree on the order of K, which is all that the sum asks for).  The eight partial sums are added in shared memory.
 // Measured from codes, back to back (us): 5 tokens 1024 x 1024 3.1, 4096 x 4096 5.3, 8192 x 8192 13.6 (67 MB of weights, 4.9 TB/s).
 // TOKENS > 0: up to that many tokens are quantised by every workgroup for itself, while its first weights are on their way: a launch less.
-constexpr int I8_STRIP_WAVES = 8, I8_STRIP_THREADS = 64 * I8_STRIP_WAVES, I8_STRIP_PIECES = 4;
+constexpr int I8_STRIP_WAVES = 8, I8_STRIP_THREADS = 64 * I8_STRIP_WAVES, I8_STRIP_VALUES = 32;      // values of x that a thread holds
 
 // TOKENS rows of x into codes [TOKENS][Kp] and scales in shared memory; 512 / TOKENS threads a row
 template <int TOKENS, bool WIDE>
 __device__ __forceinline__ void i8_strip_quantize(const I8Problem& p, const void* x, int64_t ldx, int type, int8_t* codes, int Kp, float* scale, float* red,
                                                   int* reds) {
-    constexpr int V = WIDE ? 4 : 8, TPT = I8_STRIP_THREADS / TOKENS, WPT = TPT / 64;
+    constexpr int V = WIDE ? 4 : 8, C = I8_STRIP_VALUES / V, TPT = I8_STRIP_THREADS / TOKENS, WPT = TPT / 64;
     const int tid = threadIdx.x, m = tid / TPT, t = tid % TPT, wave = tid >> 6;
     const char* base = (const char*)x + (size_t)min(m, p.M - 1) * ldx * (16 / V);
-    uint4 raw[I8_STRIP_PIECES];
+    uint4 raw[C];
     float top = 0.f;
     bool odd = false;
 #pragma unroll
-    for (int c = 0; c < I8_STRIP_PIECES; ++c) raw[c] = i8_piece<WIDE>(base, (c * TPT + t) * V, p.K);
+    for (int c = 0; c < C; ++c) raw[c] = i8_piece<WIDE>(base, (c * TPT + t) * V, p.K);
 #pragma unroll
-    for (int c = 0; c < I8_STRIP_PIECES; ++c) {
+    for (int c = 0; c < C; ++c) {
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -488,18 +488,22 @@ __device__ __forceinline__ void i8_strip_quantize(const I8Problem& p, const void
             top = fmaxf(top, fabsf(f));
         }
     }
-    top = wave_max(top);
-    const int bad = __any(odd);
-    if ((tid & 63) == 0) { red[wave] = top; reds[wave] = bad; }
-    __syncthreads();
-    float all = 0.f;
-    int any = 0;
+    int bad = odd;
 #pragma unroll
-    for (int q = 0; q < WPT; ++q) { all = fmaxf(all, red[m * WPT + q]); any |= reds[m * WPT + q]; }
-    const I8Row r = i8_row(all, any != 0);
+    for (int o = TPT < 64 ? TPT / 2 : 32; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, o));
+        bad |= __shfl_xor(bad, o);
+    }
+    if (WPT > 1) {                        // several waves hold the token
+        if ((tid & 63) == 0) { red[wave] = top; reds[wave] = bad; }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < WPT; ++q) { top = fmaxf(top, red[m * WPT + q]); bad |= reds[m * WPT + q]; }
+    }
+    const I8Row r = i8_row(top, bad != 0);
     if (t == 0) scale[m] = r.scale;
 #pragma unroll
-    for (int c = 0; c < I8_STRIP_PIECES; ++c) {
+    for (int c = 0; c < C; ++c) {
         const int k = (c * TPT + t) * V;
         if (k >= Kp) break;
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
@@ -657,16 +661,19 @@ static void launch_i8_strip_tokens(const I8Problem& p, const void* x, int64_t ld
     hipLaunchKernelGGL((gemm_i8_strip_kernel<1, 1, TOKENS>), dim3((p.N + 15) / 16), dim3(I8_STRIP_THREADS), lds, s, p, x, ldx, xtype);
 }
 
-// Up to four tokens whose values fit four pieces of 16 bytes a thread.
-bool linear_i8_fused(int xtype, int M, int K) {
-    const int V = xtype == FBHIP_F32 ? 4 : 8, rows = M == 3 ? 4 : M;
-    return M <= 4 && (K + 127) / 128 * 128 <= I8_STRIP_THREADS / rows * V * I8_STRIP_PIECES;
-}
+// Up to 16 tokens (as 1, 2, 4, 8 or 16) whose values fit 32 a thread: quantising them in every workgroup takes as long as the launch that it saves.
+static int i8_tokens(int M) { return M <= 2 ? M : M <= 4 ? 4 : M <= 8 ? 8 : 16; }
+
+bool linear_i8_fused(int M, int K) { return M <= 16 && (K + 127) / 128 * 128 <= I8_STRIP_THREADS / i8_tokens(M) * I8_STRIP_VALUES; }
 
 hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
-    if (p.M == 1) launch_i8_strip_tokens<1>(p, x, ldx, xtype, s);
-    else if (p.M == 2) launch_i8_strip_tokens<2>(p, x, ldx, xtype, s);
-    else launch_i8_strip_tokens<4>(p, x, ldx, xtype, s);
+    switch (i8_tokens(p.M)) {
+        case 1: launch_i8_strip_tokens<1>(p, x, ldx, xtype, s); break;
+        case 2: launch_i8_strip_tokens<2>(p, x, ldx, xtype, s); break;
+        case 4: launch_i8_strip_tokens<4>(p, x, ldx, xtype, s); break;
+        case 8: launch_i8_strip_tokens<8>(p, x, ldx, xtype, s); break;
+        default: launch_i8_strip_tokens<16>(p, x, ldx, xtype, s);
+    }
     return hipGetLastError();
 }
 

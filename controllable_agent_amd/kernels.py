@@ -327,7 +327,7 @@ def linear_i8(x: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, *, bias: 
     if M == 0 or N == 0:
         return y
     lib = _lib.load()
-    need = lib.fbhip_linear_i8_workspace(code, M, N, K)
+    need = lib.fbhip_linear_i8_workspace(M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     check(lib.fbhip_linear_i8(x.data_ptr(), ldx, code, W.data_ptr(), ldw, w_scale.data_ptr(), ptr(bias), int(relu), y.data_ptr(), ldy,
                               _TYPE_CODE[y.dtype], M, N, K, ptr(ws), stream))

@@ -530,7 +530,7 @@ size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K);
 int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                   int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);
 /* The same with x quantised row by row on the way (fbhip_quantize_rows into the workspace). */
-size_t fbhip_linear_i8_workspace(int32_t x_type, int32_t M, int32_t N, int32_t K);      /* 0: one launch does both */
+size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K);      /* 0: one launch does both */
 int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                     int32_t relu, void* y, int64_t ldy, int32_t y_type, int32_t M, int32_t N, int32_t K, void* workspace, void* stream);
 

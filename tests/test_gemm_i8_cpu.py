@@ -81,6 +81,8 @@ def test_c_entries_refuse_bad_calls():
         return lib.fbhip_quantize_rows(x, ldx, xt, q, ldq, s, rows, k, kp, None)
     assert all(r == -1 for r in (quant(x=None), quant(q=None), quant(s=None), quant(rows=0), quant(k=0), quant(kp=19), quant(ldq=31), quant(ldx=19),
                                  quant(xt=5)))
-    assert lib.fbhip_linear_i8_workspace(0, 40, 4, 20) >= 40 * 128 + 160 and lib.fbhip_linear_i8_workspace(0, 0, 4, 20) == 0
-    # up to four tokens of a row that fits: one launch, which needs none
-    assert lib.fbhip_linear_i8_workspace(0, 4, 4, 20) == 0 and lib.fbhip_linear_i8_workspace(0, 4, 4, 20000) > 0
+    assert lib.fbhip_linear_i8_workspace(40, 4, 20) >= 40 * 128 + 160 and lib.fbhip_linear_i8_workspace(0, 4, 20) == 0
+    # few tokens whose values fit one launch: it needs none
+    for tokens, most in ((1, 16384), (2, 8192), (3, 4096), (4, 4096), (5, 2048), (8, 2048), (9, 1024), (16, 1024)):
+        assert lib.fbhip_linear_i8_workspace(tokens, 4, most) == 0 and lib.fbhip_linear_i8_workspace(tokens, 4, most + 1) > 0
+    assert lib.fbhip_linear_i8_workspace(17, 4, 16) > 0

@@ -150,7 +150,7 @@ def test_quantize_ties_and_extremes(K):
     assert (q[3] == 0).all() and (q[8] == 0).all() and s[8] == 0 and q[1, 0] == 127 and q[1, 1] == -127 and q[5, 7] == -127
 
 
-@pytest.mark.parametrize("M", [1, 3, 20, 200])
+@pytest.mark.parametrize("M", [1, 2, 3, 7, 16, 20, 200])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_rows_that_hold_no_numbers(K, M, bad):
     """they come back as NaN, whatever the others hold; rows of zeros give the bias"""
@@ -172,9 +172,9 @@ def test_rows_that_hold_no_numbers(K, M, bad):
 
 
 # ------------------------------------------------------------------------------------------------------------------------------ linear
-@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 16, 17, 48, 64, 65, 300])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9, 13, 16, 17, 48, 64, 65, 300])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("N,Kd", [(6, 30), (526, 1051), (1024, 1024), (64, 8200), (40, 33000)])
+@pytest.mark.parametrize("N,Kd", [(6, 30), (526, 1051), (1024, 1024), (64, 8200), (40, 33000), (20, 2048), (33, 4097)])
 def test_linear_equals_quantize_then_product(K, M, N, Kd, dtype):
     gen = torch.Generator().manual_seed(M + N)
     x = torch.randn(M, Kd, generator=gen).to(dtype).cuda()
