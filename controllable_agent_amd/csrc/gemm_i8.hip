@@ -18,12 +18,6 @@ typedef uint32_t uintx4_any __attribute__((ext_vector_type(4), aligned(2)));
 constexpr int I8_BK = 128;                    // bytes of K in a step: one row of a tile is one 128-byte line
 
 // ------------------------------------------------------------------------------------------------------------------ quantiser
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
-}
-
 __device__ __forceinline__ float i8_load(const void* x, size_t i, int type) {
     if (type == FBHIP_F32) return ((const float*)x)[i];
     const uint16_t h = ((const uint16_t*)x)[i];
@@ -33,28 +27,51 @@ __device__ __forceinline__ float i8_load(const void* x, size_t i, int type) {
     return (float)f;
 }
 
-// The code of x in a row of scale s: x / s, rounded to float32 and then to the nearest whole number, ties to even.  x times the reciprocal is off by
-// less than 5e-5 for |x / s| <= 127 (a step of v_rcp_f32, half a step of the product and of the quotient: 127 * 2.5 * 2^-23 = 3.8e-5), so that only
-// a value that comes so near to a half is divided.  Scales below 2^-100 (the reciprocal would leave the range) are divided always.
-__device__ __forceinline__ int i8_code(float x, float s, float inv) {
-    const float q = x * inv;
-    float r = rintf(q);
-    if (!(fabsf(q - r) < 0.49995f)) r = fminf(fmaxf(rintf(x / s), -127.f), 127.f);
-    return (int)r;
+// The largest magnitude is found on the bits, which order like the values; infinities and NaN come out above every number.
+__device__ __forceinline__ uint32_t i8_top(uint32_t top, float x) { return max(top, __float_as_uint(x) & 0x7FFFFFFFu); }
+
+// over groups of LANES lanes
+template <int LANES>
+__device__ __forceinline__ uint32_t i8_lanes_top(uint32_t top) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    return top;
 }
 
-struct I8Row { float scale, inv; bool zero; };
+struct I8Row { float scale, inv; bool zero, divide; };
 // a row that holds a NaN or an infinity: the scale NaN and codes 0; a row of zeros, or one so small that its scale is 0: codes 0
-__device__ __forceinline__ I8Row i8_row(float top, bool bad) {
+__device__ __forceinline__ I8Row i8_row(uint32_t top) {
     I8Row r;
-    r.scale = top * (1.f / 127.f);                        // (the reciprocal rounded to float32: within a step of the quotient)
+    const bool bad = top >= 0x7F800000u;
+    r.scale = __uint_as_float(top) * (1.f / 127.f);       // (the reciprocal rounded to float32: within a step of the quotient)
     r.zero = bad || r.scale == 0.f;
-    r.inv = r.scale >= 0x1p-100f ? __builtin_amdgcn_rcpf(r.scale) : __uint_as_float(0x7FC00000u);
+    r.divide = r.scale < 0x1p-100f;                       // (the reciprocal would leave the range)
+    r.inv = r.divide ? 1.f : __builtin_amdgcn_rcpf(r.scale);
     if (bad) r.scale = __uint_as_float(0x7FC00000u);
     return r;
 }
 
-__device__ __forceinline__ bool i8_no_number(float x) { return !(fabsf(x) < __uint_as_float(0x7F800000u)); }
+// The codes of four values: x / s, rounded to float32 and then to the nearest whole number, ties to even.  x times the reciprocal is off by less than
+// 5e-5 for |x / s| <= 127 (a step of v_rcp_f32, half a step of the product and of the quotient: 127 * 2.5 * 2^-23 = 3.8e-5), so that only where
+// a value comes so near to a half the four are divided.  The conversion packs bytes of 0..255: 128 is added, and taken off in the top bits.
+__device__ __forceinline__ uint32_t i8_codes(float a, float b, float c, float d, const I8Row& r) {
+    const float x[4] = {a, b, c, d};
+    float n[4], off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float q = x[e] * r.inv;
+        n[e] = rintf(q);
+        off = fmaxf(off, fabsf(q - n[e]));
+    }
+    if (off >= 0.49995f || r.divide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n[e] = fminf(fmaxf(rintf(x[e] / r.scale), -127.f), 127.f);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w = __builtin_amdgcn_cvt_pk_u8_f32(n[e] + 128.f, e, w);
+    return r.zero ? 0u : w ^ 0x80808080u;
+}
 
 // values e of a 16-byte piece
 template <bool WIDE>
@@ -89,53 +106,40 @@ template <int TPR, int C, bool WIDE>
 __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
                                                                 float* __restrict__ scale, int rows, int K, int Kp) {
     constexpr int V = WIDE ? 4 : 8;                       // values of a piece (WIDE: fp32)
-    __shared__ float red[4];
-    __shared__ int reds[4];
+    __shared__ uint32_t red[4];
     const int t = threadIdx.x % TPR, row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const bool live = row < rows;                         // (only TPR = 64 has rows behind the end)
     const char* base = (const char*)x + (size_t)(live ? row : rows - 1) * ldx * (16 / V);
     float v[C][V];
-    float top = 0.f;
-    bool odd = false;
+    uint32_t top = 0;
     uint4 raw[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        raw[c] = i8_piece<WIDE>(base, (c * TPR + t) * V, K);
-    }
+    for (int c = 0; c < C; ++c) raw[c] = i8_piece<WIDE>(base, (c * TPR + t) * V, K);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float f = i8_unpack<WIDE>(w, e, type);
-            v[c][e] = f;
-            odd = odd || i8_no_number(f);
-            top = fmaxf(top, fabsf(f));
+            v[c][e] = i8_unpack<WIDE>(w, e, type);
+            top = i8_top(top, v[c][e]);
         }
     }
-    top = wave_max(top);
-    int bad = __any(odd);
+    top = i8_lanes_top<64>(top);
     if (TPR == 256) {
-        if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = top; reds[threadIdx.x >> 6] = bad; }
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
         __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        bad = reds[0] | reds[1] | reds[2] | reds[3];
+        top = max(max(red[0], red[1]), max(red[2], red[3]));
     }
-    const I8Row r = i8_row(top, bad != 0);
+    const I8Row r = i8_row(top);
     if (!live) return;
     int8_t* out = q + (size_t)row * ldq;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k = (c * TPR + t) * V;
         if (k >= Kp) break;
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int code = r.zero ? 0 : i8_code(v[c][e], r.scale, r.inv);      // (zeros behind K stay zeros)
-            w[e >> 2] |= (uint32_t)(code & 0xFF) << (8 * (e & 3));
-        }
-        if (WIDE) *(uint32_t*)(out + k) = w[0];
-        else *(uint2*)(out + k) = make_uint2(w[0], w[1]);
+        const uint32_t first = i8_codes(v[c][0], v[c][1], v[c][2], v[c][3], r);          // (zeros behind K stay zeros)
+        if (WIDE) *(uint32_t*)(out + k) = first;
+        else *(uint2*)(out + k) = make_uint2(first, i8_codes(v[c][V - 4], v[c][V - 3], v[c][V - 2], v[c][V - 1], r));
     }
     if (t == 0) scale[row] = r.scale;
 }
@@ -143,24 +147,17 @@ __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __re
 // Longer rows: a workgroup reads them twice.
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
                                                             float* __restrict__ scale, int K, int Kp) {
-    __shared__ float red[4];
-    __shared__ int reds[4];
+    __shared__ uint32_t red[4];
     const int tid = threadIdx.x;
     const size_t base = (size_t)blockIdx.x * ldx;
-    float top = 0.f;
-    bool odd = false;
-    for (int k = tid; k < K; k += 256) {
-        const float v = i8_load(x, base + k, type);
-        odd = odd || i8_no_number(v);
-        top = fmaxf(top, fabsf(v));
-    }
-    top = wave_max(top);
-    const int bad = __any(odd);
-    if ((tid & 63) == 0) { red[tid >> 6] = top; reds[tid >> 6] = bad; }
+    uint32_t top = 0;
+    for (int k = tid; k < K; k += 256) top = i8_top(top, i8_load(x, base + k, type));
+    top = i8_lanes_top<64>(top);
+    if ((tid & 63) == 0) red[tid >> 6] = top;
     __syncthreads();
-    const I8Row r = i8_row(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), (reds[0] | reds[1] | reds[2] | reds[3]) != 0);
+    const I8Row r = i8_row(max(max(red[0], red[1]), max(red[2], red[3])));
     for (int k = tid; k < Kp; k += 256)
-        q[(size_t)blockIdx.x * ldq + k] = (int8_t)(k < K && !r.zero ? i8_code(i8_load(x, base + k, type), r.scale, r.inv) : 0);
+        q[(size_t)blockIdx.x * ldq + k] = (int8_t)(k < K ? i8_codes(i8_load(x, base + k, type), 0.f, 0.f, 0.f, r) & 0xFFu : 0u);
     if (tid == 0) scale[blockIdx.x] = r.scale;
 }
 
@@ -466,52 +463,41 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
 // TOKENS > 0: up to that many tokens are quantised by every workgroup for itself, while its first weights are on their way: a launch less.
 constexpr int I8_STRIP_WAVES = 8, I8_STRIP_THREADS = 64 * I8_STRIP_WAVES, I8_STRIP_VALUES = 32;      // values of x that a thread holds
 
-// TOKENS rows of x into codes [TOKENS][Kp] and scales in shared memory; 512 / TOKENS threads a row
+// TOKENS rows of x into codes [TOKENS][Kp] and scales in shared memory; 512 / TOKENS threads a row, I8_STRIP_VALUES values a thread
 template <int TOKENS, bool WIDE>
-__device__ __forceinline__ void i8_strip_quantize(const I8Problem& p, const void* x, int64_t ldx, int type, int8_t* codes, int Kp, float* scale, float* red,
-                                                  int* reds) {
+__device__ __forceinline__ void i8_strip_quantize(const I8Problem& p, const void* x, int64_t ldx, int type, int8_t* codes, int Kp, float* scale,
+                                                  uint32_t* red) {
     constexpr int V = WIDE ? 4 : 8, C = I8_STRIP_VALUES / V, TPT = I8_STRIP_THREADS / TOKENS, WPT = TPT / 64;
-    const int tid = threadIdx.x, m = tid / TPT, t = tid % TPT, wave = tid >> 6;
+    const int tid = threadIdx.x, m = tid / TPT, t = tid % TPT;
     const char* base = (const char*)x + (size_t)min(m, p.M - 1) * ldx * (16 / V);
     uint4 raw[C];
-    float top = 0.f;
-    bool odd = false;
+    uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c) raw[c] = i8_piece<WIDE>(base, (c * TPT + t) * V, p.K);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float f = i8_unpack<WIDE>(w, e, type);
-            odd = odd || i8_no_number(f);
-            top = fmaxf(top, fabsf(f));
-        }
+        for (int e = 0; e < V; ++e) top = i8_top(top, i8_unpack<WIDE>(w, e, type));
     }
-    int bad = odd;
-#pragma unroll
-    for (int o = TPT < 64 ? TPT / 2 : 32; o > 0; o >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, o));
-        bad |= __shfl_xor(bad, o);
-    }
+    top = i8_lanes_top<TPT < 64 ? TPT : 64>(top);
     if (WPT > 1) {                        // several waves hold the token
-        if ((tid & 63) == 0) { red[wave] = top; reds[wave] = bad; }
+        if ((tid & 63) == 0) red[tid >> 6] = top;
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < WPT; ++q) { top = fmaxf(top, red[m * WPT + q]); bad |= reds[m * WPT + q]; }
+        for (int q = 0; q < WPT; ++q) top = max(top, red[m * WPT + q]);
     }
-    const I8Row r = i8_row(top, bad != 0);
+    const I8Row r = i8_row(top);
     if (t == 0) scale[m] = r.scale;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k = (c * TPT + t) * V;
         if (k >= Kp) break;
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-        uint32_t o[2] = {0u, 0u};
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e >> 2] |= (uint32_t)((r.zero ? 0 : i8_code(i8_unpack<WIDE>(w, e, type), r.scale, r.inv)) & 0xFF) << (8 * (e & 3));
-        if (WIDE) *(uint32_t*)(codes + m * Kp + k) = o[0];
-        else *(uint2*)(codes + m * Kp + k) = make_uint2(o[0], o[1]);
+        for (int e = 0; e < V; e += 4)
+            *(uint32_t*)(codes + m * Kp + k + e) = i8_codes(i8_unpack<WIDE>(w, e, type), i8_unpack<WIDE>(w, e + 1, type), i8_unpack<WIDE>(w, e + 2, type),
+                                                            i8_unpack<WIDE>(w, e + 3, type), r);
     }
     __syncthreads();
 }
@@ -521,8 +507,8 @@ __global__ void __launch_bounds__(I8_STRIP_THREADS) gemm_i8_strip_kernel(const I
     static_assert(TOKENS <= 16 && (TOKENS == 0 || MT == 1), "quantised tokens fit one tile");
     extern __shared__ __attribute__((aligned(16))) int8_t codes[];         // TOKENS > 0: [TOKENS][Kp]
     __shared__ __attribute__((aligned(16))) intx4 part[I8_STRIP_WAVES][NT * MT][64];
-    __shared__ float token_scale[16], red[I8_STRIP_WAVES];
-    __shared__ int reds[I8_STRIP_WAVES];
+    __shared__ float token_scale[16];
+    __shared__ uint32_t red[I8_STRIP_WAVES];
     constexpr int DEEP = NT * MT >= 4 ? 2 : 4;                // chunks whose loads are under way together
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, quarter = lane >> 4;
     const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT, K = p.K, chunks = (K + 127) / 128, k16 = (K + 15) & ~15, Kp = chunks * 128;
@@ -550,8 +536,8 @@ __global__ void __launch_bounds__(I8_STRIP_THREADS) gemm_i8_strip_kernel(const I
     };
     load(wave);
     if (TOKENS) {
-        if (xtype == FBHIP_F32) i8_strip_quantize<TOKENS ? TOKENS : 1, true>(p, x, ldx, xtype, codes, Kp, token_scale, red, reds);
-        else i8_strip_quantize<TOKENS ? TOKENS : 1, false>(p, x, ldx, xtype, codes, Kp, token_scale, red, reds);
+        if (xtype == FBHIP_F32) i8_strip_quantize<TOKENS ? TOKENS : 1, true>(p, x, ldx, xtype, codes, Kp, token_scale, red);
+        else i8_strip_quantize<TOKENS ? TOKENS : 1, false>(p, x, ldx, xtype, codes, Kp, token_scale, red);
     }
     for (int c0 = wave; c0 < chunks; c0 += I8_STRIP_WAVES * DEEP) {
         intx4 a[DEEP][MT][2];
@@ -655,26 +641,27 @@ static void launch_i8_strip(const I8Problem& p, hipStream_t s) {
                        nullptr, (int64_t)0, (int)FBHIP_F32);
 }
 
-template <int TOKENS>
-static void launch_i8_strip_tokens(const I8Problem& p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
-    const size_t lds = (size_t)TOKENS * ((p.K + 127) / 128 * 128);
-    hipLaunchKernelGGL((gemm_i8_strip_kernel<1, 1, TOKENS>), dim3((p.N + 15) / 16), dim3(I8_STRIP_THREADS), lds, s, p, x, ldx, xtype);
-}
-
-// Up to 16 tokens (as 1, 2, 4, 8 or 16) whose values fit 32 a thread: quantising them in every workgroup takes as long as the launch that it saves.
+// Up to 16 tokens (as 1, 2, 4, 8 or 16) whose values fit I8_STRIP_VALUES a thread are quantised by every workgroup of the product.  With 128 values a
+// thread more of them fit, but 4 tokens of 8192 values took 29 us in one launch and 18 in two.
 static int i8_tokens(int M) { return M <= 2 ? M : M <= 4 ? 4 : M <= 8 ? 8 : 16; }
 
-bool linear_i8_fused(int M, int K) { return M <= 16 && (K + 127) / 128 * 128 <= I8_STRIP_THREADS / i8_tokens(M) * I8_STRIP_VALUES; }
+bool linear_i8_fused(int M, int K) { return M <= 16 && K <= I8_STRIP_VALUES * I8_STRIP_THREADS / i8_tokens(M); }
+
+template <int TOKENS>
+static hipError_t launch_i8_strip_tokens(const I8Problem& p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
+    const size_t lds = (size_t)TOKENS * ((p.K + 127) / 128 * 128);         // at most I8_STRIP_VALUES * I8_STRIP_THREADS bytes
+    hipLaunchKernelGGL((gemm_i8_strip_kernel<1, 1, TOKENS>), dim3((p.N + 15) / 16), dim3(I8_STRIP_THREADS), lds, s, p, x, ldx, xtype);
+    return hipGetLastError();
+}
 
 hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int xtype, hipStream_t s) {
     switch (i8_tokens(p.M)) {
-        case 1: launch_i8_strip_tokens<1>(p, x, ldx, xtype, s); break;
-        case 2: launch_i8_strip_tokens<2>(p, x, ldx, xtype, s); break;
-        case 4: launch_i8_strip_tokens<4>(p, x, ldx, xtype, s); break;
-        case 8: launch_i8_strip_tokens<8>(p, x, ldx, xtype, s); break;
-        default: launch_i8_strip_tokens<16>(p, x, ldx, xtype, s);
+        case 1: return launch_i8_strip_tokens<1>(p, x, ldx, xtype, s);
+        case 2: return launch_i8_strip_tokens<2>(p, x, ldx, xtype, s);
+        case 4: return launch_i8_strip_tokens<4>(p, x, ldx, xtype, s);
+        case 8: return launch_i8_strip_tokens<8>(p, x, ldx, xtype, s);
+        default: return launch_i8_strip_tokens<16>(p, x, ldx, xtype, s);
     }
-    return hipGetLastError();
 }
 
 hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s) {
