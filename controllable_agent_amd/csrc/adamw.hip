@@ -8,8 +8,9 @@
 // written once; a lane holds eight consecutive elements, so that each 16-bit stream is one 16-byte access, an fp32 one two and a code
 // stream one of 8 bytes, and a block of 256 elements that shares a scale is half a wave: its maximum is five lane exchanges.  (Four elements a
 // lane leave room for more waves and take 20 % longer: the accesses are half as wide.)
-// Measured, on a card whose large copy reaches 4.93 TB/s: 134 M fp32 parameters, bf16 gradients, 8-bit moments 372 us (5.07 TB/s); 67 M in bf16 with
-// fp32 moments 282 us (5.2 TB/s) and 27 us for their norm (5.0 TB/s); 3.7 M in fp32 22 us (32 bits), 17 us (8 bits), of which the start of
+// Measured, on a card whose large copy reaches 4.93 TB/s: 134 M fp32 parameters, bf16 gradients, 8-bit moments 376 us (5.02 TB/s); 67 M in bf16 with
+// fp32 moments and their norm 324 us (4.96 TB/s; alone in a trace 268 and 56, of which the norm shares half with the last step's writes that leave the
+// cache: more loads under way in it gained 1 % there and lost 10 % on 3.7 M); 3.7 M in fp32 21 us (32 bits), 17 us (8 bits), of which the start of
 // a workgroup (scalars, tables, first loads) is a third.
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 codes times a power of two for each 256 elements (the least one under which the

@@ -284,7 +284,7 @@ struct I8Tile {
 // 1 KB of global memory into shared memory, lane l's 16 bytes behind lane l-1's.  (Assembly: the compiler would wait for all such
 // loads in front of every read of shared memory; no register is written.)
 __device__ __forceinline__ void i8_load_lds(uint32_t lds, uint32_t offset, const void* base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 
 template <int COUNT>
