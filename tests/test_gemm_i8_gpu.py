@@ -150,6 +150,23 @@ def test_quantize_ties_and_extremes(K):
     assert (q[3] == 0).all() and (q[8] == 0).all() and s[8] == 0 and q[1, 0] == 127 and q[1, 1] == -127 and q[5, 7] == -127
 
 
+@pytest.mark.parametrize("rows", [1, 16, 400])
+def test_codes_beside_the_halves(K, rows):
+    """quotients within a few steps of a half, on scales from 2^-118 to 2^110: the code is the rounded quotient's, in the quantiser and in the product
+    (127 times the identity hands the codes back: six roundings of half a step lie between them and code * scale, 4e-7; a wrong code is off by 1/127)"""
+    gen = torch.Generator().manual_seed(rows)
+    scale = torch.exp2(torch.rand(rows, 1, generator=gen) * 228 - 118)
+    half = (torch.randint(-127, 127, (rows, 255), generator=gen) + 0.5) * scale
+    steps = torch.randint(-4, 5, half.shape, generator=gen, dtype=torch.int32)
+    x = torch.cat([127 * scale, (half.view(torch.int32) + steps).view(torch.float32)], 1)
+    q, s = K.quantize_rows(x.cuda())
+    want, ws = _want_codes(x)
+    assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), want)
+    eye, one = K.quantize_rows(torch.eye(256, device="cuda") * 127)
+    y = K.linear_i8(x.cuda(), eye, one / 127)
+    assert torch.allclose(y.cpu().double() / ws.double()[:, None], want.double(), rtol=1e-5, atol=0)
+
+
 @pytest.mark.parametrize("M", [1, 2, 3, 7, 16, 20, 200])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_rows_that_hold_no_numbers(K, M, bad):
