@@ -8,17 +8,18 @@
 // written once; a lane holds eight consecutive elements, so that each 16-bit stream is one 16-byte access, an fp32 one two and a code
 // stream one of 8 bytes, and a block of 256 elements that shares a scale is half a wave: its maximum is five lane exchanges.  (Four elements a
 // lane leave room for more waves and take 20 % longer: the accesses are half as wide.)
-// Measured, on a card whose large copy reaches 4.93 TB/s: 134 M fp32 parameters, bf16 gradients, 8-bit moments 376 us (5.02 TB/s); 67 M in bf16 with
-// fp32 moments and their norm 324 us (4.96 TB/s; alone in a trace 268 and 56, of which the norm shares half with the last step's writes that leave the
-// cache: more loads under way in it gained 1 % there and lost 10 % on 3.7 M); 3.7 M in fp32 21 us (32 bits), 17 us (8 bits), of which the start of
-// a workgroup (scalars, tables, first loads) is a third.
+// Measured, on a card whose large copy reaches 4.93 TB/s: 134 M fp32 parameters, bf16 gradients, 8-bit moments 422 us (4.47 TB/s, the arithmetic shows);
+// 67 M in bf16 with fp32 moments and their norm 329 us (4.89 TB/s; more loads under way in the norm gained 1 % there and lost 10 % on 3.7 M); 3.7 M in
+// fp32 21 us (32 bits), 23 us (8 bits and the norm), of which the start of a workgroup (scalars, tables, first loads) is a third.
+// Root and quotient are correctly rounded, as the plain form's are.  With the instructions that are good to a step (v_sqrt_f32, v_rcp_f32) these took 380,
+// 325, 21 and 22 us, but parameters differed in their last bit from the formulas' single-precision operations, and now and then a code of r by a step.
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 codes times a power of two for each 256 elements (the least one under which the
 // block's largest magnitude is at most 448).  r, not v: the step divides by sqrt(v), and the root halves the range that the codes have to
 // span.  Codes are rounded up or down at random so that their mean is the value: a step moves v by a thousandth (1 - b2), half a code step
 // is 3 %, and nearest rounding would never move r at all.  A positive r never rounds to zero (the update would divide by eps alone).
-// The arithmetic before the codes is written without contraction, so that a code depends on single-precision operations in the order of
-// the formulas and on nothing else.  A value that is no number keeps its own code (NaN) and does not touch the block's scale.
+// The arithmetic before the codes is written without contraction and correctly rounded, so that a code depends on single-precision operations in the order
+// of the formulas and on nothing else.  A value that is no number keeps its own code (NaN) and does not touch the block's scale.
 #include "common.h"
 #include "fbhip.h"
 
@@ -285,22 +286,10 @@ __global__ void __launch_bounds__(ADAMW_THREADS, 5) adamw_kernel(const AdamwArgs
             m[j] = m[j] + w1 * (gr - m[j]);
             v[j] = v[j] * b2 + (w2 * gr) * gr;
         }
-        // The square root's instruction is good to one step, for normal numbers; so is the reciprocal's (the denominator is none or normal: the root of
-        // the least number is 3.7e-23)
-        uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            r[j] = __builtin_amdgcn_sqrtf(v[j]);
-            least = min(least, __float_as_uint(v[j]) - 1u);
-        }
-        if (least < 0x7FFFFFu) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) r[j] = sqrtf(v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float den = r[j] * rbc2 + eps;
-            p[j] = p[j] * keep - ss * (m[j] * __builtin_amdgcn_rcpf(den));
+            r[j] = sqrtf(v[j]);
+            p[j] = p[j] * keep - ss * (m[j] / (r[j] * rbc2 + eps));
         }
         uint32_t word[8];
         if (BITS == 8 || T.dtype == FBHIP_BF16) element_words(s, key, word);
