@@ -41,11 +41,11 @@ hipError_t launch_stream(hipStream_t* out) {
     return hipSuccess;
 }
 
-// May this process replay graphs with parallel branches at all?  The guard above is verified by runs, for the HIP 7.0 runtime that torch
-// 2.10 bundles; HIP 7.2 came through without it.  So: branched graphs on HIP 7.0.x (with the guard) and on HIP >= 7.2, provided the
-// device has a high-priority class; on any other runtime the library REFUSES them and builds its n-step graphs single-queue (the plain
-// form: same kernels and results, 3-6 % slower) instead of silently running the configuration that crashed.  FBHIP_BRANCHED_GRAPHS=1
-// forces them on an unlisted runtime, =0 refuses them everywhere (read at every call: tests force the fallback with it).
+// May this process replay graphs with parallel branches at all?  The guard above is verified by runs, and those were made on the HIP 7.0
+// runtime that torch 2.10 bundles only.  So: branched graphs on HIP 7.0.x (with the guard), provided the device has a high-priority
+// class; on any other runtime the library REFUSES them and builds its n-step graphs single-queue (the plain form: same kernels and
+// results, 3-6 % slower) instead of silently running the configuration that crashed.  FBHIP_BRANCHED_GRAPHS=1 forces them on an
+// unlisted runtime, =0 refuses them everywhere (read at every call: tests force the fallback with it).
 const char* branched_graphs_verdict(bool* ok) {
     static const char* cached = nullptr;
     static bool cached_ok = false;
@@ -56,7 +56,6 @@ const char* branched_graphs_verdict(bool* ok) {
         if (hipDeviceGetStreamPriorityRange(&lo, &hi) != hipSuccess || hi >= lo) { (void)hipGetLastError(); cached = "refused: the device has no high-priority stream class"; return; }
         const int major = v / 10000000, minor = (v / 100000) % 100;
         if (major == 7 && minor == 0) { cached_ok = true; cached = "allowed: HIP 7.0 runtime, launched from a high-priority stream (verified workaround)"; }
-        else if (major > 7 || (major == 7 && minor >= 2)) { cached_ok = true; cached = "allowed: HIP >= 7.2 runtime"; }
         else cached = "refused: unverified HIP runtime version for graphs with parallel branches (FBHIP_BRANCHED_GRAPHS=1 forces them)";
     });
     const char* e = getenv("FBHIP_BRANCHED_GRAPHS");
@@ -75,8 +74,7 @@ int launch_graph(fbhip_ctx* c, hipGraphExec_t exec, hipStream_t s, bool branches
         HIPCK(c, hipGraphLaunch(exec, s));
         return FBHIP_OK;
     }
-    {   // the caller's stream is itself of the high-priority class: its hardware queue comes from the other pool already -- launch
-        // there, without the two event hops (measured round 4, HISTORY.md: per-update launches of a branched
+    {   // the caller's stream is itself of the high-priority class: launch there, without the two event hops (measured round 4, HISTORY.md: per-update launches of a branched
         // graph run at 1108 update-steps/s this way, at 513 through the hop under the runtime's default dependency handling)
         int prio = 0, lo = 0, hi = 0;
         if (s != nullptr && hipStreamGetPriority(s, &prio) == hipSuccess && hipDeviceGetStreamPriorityRange(&lo, &hi) == hipSuccess && hi < lo && prio == hi) {

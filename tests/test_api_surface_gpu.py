@@ -14,10 +14,10 @@ from oracle import sf_oracle as so
 from tests import helpers as H
 
 # (Round 2 ran these 37 cases in a process of their own: with them in the main pytest process an intermittent segfault appeared
-# inside LATER tests' first multi-step graph launch.  Round 3 found the cause -- ROCm 7.0's hipGraphLaunch walks off the exec's
-# parallel-stream list when both of a two-branch graph's runtime-internal streams share the launch stream's hardware queue, which
-# the stream churn of ~110 short-lived contexts makes likely -- and the library now launches such graphs from a high-priority
-# stream (csrc/api.hip::launch_graph; tools/graph_queue_collision.hip reproduces it).  The cases are back in the main process.)
+# inside LATER tests' first multi-step graph launch.  On ROCm 7.0 hipGraphLaunch of a graph with parallel branches can end the
+# process when it is launched from a normal-priority stream, after the stream churn of ~110 short-lived contexts in about one run
+# in three; from a high-priority stream it never did, and the library now launches such graphs from one
+# (csrc/api.hip::launch_graph).  The cases are back in the main process.)
 pytestmark = pytest.mark.gpu
 BATCH_KEYS = ("obs", "action", "reward", "next_obs", "discount", "goal", "next_goal", "future_obs", "future_goal")
 
