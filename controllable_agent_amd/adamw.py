@@ -151,8 +151,7 @@ class AdamW:
                          *self.betas, self.eps)
         self._opt_ref = C.byref(self._opt)
         self._versioned = [p for p in self.params if not p.is_inference()]       # (tensors made in inference mode have no version)
-        self._seen: tp.Any = None                  # strides, sizes, types and devices that passed the checks, and what they gave
-        self._row_strided = any(cols for cols, _ in self._layouts)
+        self._seen: tp.Any = None                  # strides, shapes, types and devices that passed the checks, and what they gave
         self._types = b""
         self._set_step(0)
 
@@ -173,9 +172,10 @@ class AdamW:
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} parameters")
         try:
-            # (strides and size fix a dense tensor's shape; a row-strided matrix's is asked for)
-            seen = (list(map(torch.Tensor.stride, grads)), list(map(torch.Tensor.numel, grads)), list(map(_DTYPE, grads)),
-                    list(map(torch.Tensor.get_device, grads)), [g.shape for g in grads] if self._row_strided else None)
+            # (shapes and strides together: the same strides and size may belong to a part of a larger matrix, or to rows that overlap; what is
+            # contiguous has no strides to compare)
+            strides = None if all(map(torch.Tensor.is_contiguous, grads)) else list(map(torch.Tensor.stride, grads))
+            seen = (strides, list(map(torch.Tensor.size, grads)), list(map(_DTYPE, grads)), list(map(torch.Tensor.get_device, grads)))
         except (AttributeError, TypeError):
             raise ValueError("AdamW.step: a gradient is no tensor: leave its parameter out, or pass zeros (which decay its moments)") from None
         if seen == self._seen:                     # as in the last step

@@ -92,3 +92,18 @@ def test_smallest_and_largest_second_moments(AdamW):
     V = F(1) * G * G
     P = F(0) - F(1) * (G / (np.sqrt(V) + F(1e-30)))
     assert np.array_equal(p.cpu().numpy(), P) and np.array_equal(opt.v.cpu().numpy()[:len(g)], V)
+
+
+def test_a_second_step_refuses_what_a_first_one_does(AdamW):
+    """a gradient of the same strides, size, type and device that is not the parameter's like: part of a wider matrix"""
+    p = torch.zeros(4, 6, device="cuda")
+    opt = AdamW([p], lr=1e-2)
+    opt.step([torch.ones(4, 6, device="cuda")])
+    before = p.clone()
+    for bad in (torch.ones(8, 6, device="cuda")[:, :3], torch.ones(24, device="cuda").as_strided((3, 8), (6, 1)), torch.ones(24, device="cuda"),
+                torch.ones(4, 6), torch.ones(4, 6, device="cuda").double()):
+        with pytest.raises((ValueError, TypeError)):
+            opt.step([bad])
+    assert opt.step_count == 1 and torch.equal(p, before)
+    opt.step([torch.ones(4, 6, device="cuda", dtype=torch.float16)])
+    assert opt.step_count == 2
