@@ -6,6 +6,8 @@
 #include "common.h"
 #include "host.h"
 
+#include <atomic>
+
 namespace fbhip {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
@@ -596,9 +598,17 @@ __global__ void __launch_bounds__(I8_STRIP_THREADS) gemm_i8_strip_kernel(const I
 template <int WN, int WM, int FN, int FM, int BK, int S>
 static hipError_t launch_i8_tile(I8Problem p, int slices, hipStream_t s) {
     using T = I8Tile<WN, WM, FN, FM, BK, S>;
-    static const hipError_t prepared =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_kernel<WN, WM, FN, FM, BK, S>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-    if (prepared != hipSuccess) return prepared;
+    // the limit of dynamic shared memory belongs to the current device's copy of the kernel: it is raised once on each (twice does no harm)
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
+    if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_kernel<WN, WM, FN, FM, BK, S>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+        if (e != hipSuccess) return e;
+        ready.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+    }
     const int tiles = ((p.N + T::BN - 1) / T::BN) * ((p.M + T::BM - 1) / T::BM);
     p.steps *= I8_BK / BK;
     hipLaunchKernelGGL((gemm_i8_kernel<WN, WM, FN, FM, BK, S>), dim3(tiles, slices), dim3(T::THREADS), T::LDS, s, p);

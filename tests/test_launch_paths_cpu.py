@@ -48,3 +48,34 @@ print(lib.fbhip_branched_graphs(C.byref(why)), why.value.decode())
 """)
     got, why = out.strip().split(" ", 1)
     assert int(got) == allowed and why.startswith("allowed: HIP 7.0" if allowed else "refused: unverified"), out
+
+
+GEMM = """
+def gemm(M, N, K):
+    ld = -(-K // 16) * 16
+    return lib.fbhip_gemm_i8(P(4096), L(ld), P(4096), P(4096), L(ld), P(4096), None, I(0), P(4096), L(N), I(0), I(M), I(N), I(K), P(4096), None)
+SIZES = [(3600, 3500, 130), (2500, 1301, 333), (1500, 1500, 200), (300, 200, 200)]          # tiles of 256, 128 and 64 (two and four steps deep)
+"""
+
+
+def test_every_device_gets_the_tiles_shared_memory(run):
+    """the limit is a device's own: a process that goes on to a second device has to raise it there too, once"""
+    out = run(GEMM + """
+for device in (0, 1, 0, 7, 1):
+    hip.stand_in_device(device)
+    for size in SIZES:
+        rc = gemm(*size)
+        assert rc == 0, (device, size, rc, lib.fbhip_last_error(None))
+print(hip.stand_in_attributes(), hip.stand_in_launches())
+""")
+    assert out.split() == ["12", "20"], out          # four kernels on three devices; no K of these is split
+
+
+def test_a_refused_limit_is_asked_for_again(run):
+    run(GEMM + """
+for size in SIZES:
+    hip.stand_in_refuse_attribute(1)
+    assert gemm(*size) != 0 and lib.fbhip_last_error(None)
+    hip.stand_in_refuse_attribute(0)
+    assert gemm(*size) == 0
+""")
