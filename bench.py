@@ -314,7 +314,10 @@ def supervise_ranks(args, rank, world):
             time.sleep(1.0)
             rc = child.poll()
             last = hb.stat().st_mtime if hb.exists() else t0
-            allow = args.stall_timeout if hb.exists() else max(args.stall_timeout, 420.0)      # (a fresh box pages torch in for minutes)
+            # (a fresh box pages torch in for minutes; and between "process group up" and the agent built a rank only computes: the orthogonal
+            # initialisation of five networks on the host, 17 to 35 s where others want the same cores, and no other rank waits for it)
+            slow = not hb.exists() or hb.read_text().strip().endswith("process group up")
+            allow = max(args.stall_timeout, 420.0) if slow else args.stall_timeout
             mine_failed = (rc is not None and rc != 0) or (rc is None and time.time() - last > allow)
             st = torch.tensor([1.0 if mine_failed else 0.0, 1.0 if rc == 0 else 0.0])
             failed, done = st[:1].clone(), st[1:].clone()
@@ -347,7 +350,7 @@ def supervise_ranks(args, rank, world):
                         print(ln, file=sys.stderr)
             break
         if rank == 0:
-            print(f"bench.py: transport {tr} did not finish ({[e['outcome'] for e in every]}); "
+            print(f"bench.py: transport {tr} did not finish after {history[-1]['seconds']} s ({every}); "
                   + ("trying the next one" if attempt + 1 < len(plan) else "no transport left"), file=sys.stderr, flush=True)
     ok = [line is not None]
     dist.broadcast_object_list(ok, src=0)
@@ -450,6 +453,9 @@ def main():
     torch.cuda.set_device(local_rank)
     dev = f"cuda:{local_rank}"
     if world > 1:
+        # the ranks share the host's cores: with a thread for every core in each of two ranks the networks' initialisation (28 small QR
+        # factorisations on the host) takes 16 s and more instead of 0.3
+        torch.set_num_threads(max(1, torch.get_num_threads() // world))
         import torch.distributed as dist
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         # control plane: with the library-owned RCCL transport (the default) or the peer kernels the process group only carries the
