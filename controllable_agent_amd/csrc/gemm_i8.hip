@@ -184,9 +184,23 @@ hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q,
 }
 
 // ------------------------------------------------------------------------------------------------------------------ epilogue
-__device__ __forceinline__ float i8_value(const I8Problem& p, int acc, float sa, float sw, float bias) {
-    const float y = (float)acc * (sa * sw) + bias;          // (the scales first: their product leaves the range only where the value does)
-    return p.relu && y < 0.f ? 0.f : y;          // (NaN stays)
+// A scale whose product with any other such scale is a normal number.
+__device__ __forceinline__ bool i8_ordinary(float s) { return fabsf(s) >= 0x1p-62f && fabsf(s) <= 0x1p62f; }
+
+// Four neighbouring channels of a token.  The scales' product comes first: neither scale times the sum need be in range.  Where that product itself is no
+// normal number (a sum of 0 would make NaN of an infinite one, and a subnormal one has lost bits that a sum of up to 2^31 brings back) the scales'
+// exponents are kept apart and applied at the end.
+template <bool ORDINARY>
+__device__ __forceinline__ void i8_values(const I8Problem& p, const intx4& acc, float sa, const float (&sw)[4], const float (&bias)[4], float (&y)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float s = sa * sw[j];
+        y[j] = fmaf((float)acc[j], s, bias[j]);          // (written out: a value must not depend on which of the two forms its tile takes)
+        if (!ORDINARY && !__builtin_amdgcn_classf(s, 0x108))          // (a normal number of either sign)
+            y[j] = __builtin_amdgcn_ldexpf((float)acc[j] * (__builtin_amdgcn_frexp_mantf(sa) * __builtin_amdgcn_frexp_mantf(sw[j])),
+                                           __builtin_amdgcn_frexp_expf(sa) + __builtin_amdgcn_frexp_expf(sw[j])) + bias[j];
+        y[j] = p.relu && y[j] < 0.f ? 0.f : y[j];          // (NaN stays)
+    }
 }
 
 __device__ __forceinline__ uint32_t i8_half(float y, int type) {
@@ -226,6 +240,23 @@ __device__ __forceinline__ void i8_store4(const I8Problem& p, size_t at, int cou
     }
 }
 
+template <int COLS, bool ORDINARY>
+__device__ __forceinline__ void i8_rows_out(const I8Problem& p, const int* box, int ld, int m, int n, int rows, int cols, const float* sa, const float* sw,
+                                            const float* bias, int lane) {
+    constexpr int LANES = COLS / 4;
+    const int c = lane % LANES * 4;
+    if (c >= cols) return;
+    const float4 s4 = *(const float4*)(sw + c), b4 = *(const float4*)(bias + c);
+    const float s[4] = {s4.x, s4.y, s4.z, s4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll 4
+    for (int r = lane / LANES; r < rows; r += 64 / LANES) {
+        const intx4 v = *(const intx4*)(box + r * ld + c);
+        float y[4];
+        i8_values<ORDINARY>(p, v, sa[r], s, b, y);
+        i8_store4(p, (size_t)(m + r) * p.ldy + n + c, min(4, cols - c), y);
+    }
+}
+
 // `rows` tokens from m on, `cols` channels from n on (at most 32 x COLS), their sums in shared memory; the scales and the bias in shared memory too
 template <int COLS>
 __device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int ld, int m, int n, int rows, int cols, const float* sa, const float* sw,
@@ -240,17 +271,12 @@ __device__ __forceinline__ void i8_rows(const I8Problem& p, const int* box, int 
             for (int r = lane / LANES; r < rows; r += 64 / LANES) *(intx4*)(o + (size_t)r * ldp + c) = *(const intx4*)(box + r * ld + c);
         return;
     }
-    constexpr int LANES = COLS / 4;
-    const int c = lane % LANES * 4;
-    if (c >= cols) return;
-    const float4 s = *(const float4*)(sw + c), b = *(const float4*)(bias + c);
-#pragma unroll 4
-    for (int r = lane / LANES; r < rows; r += 64 / LANES) {
-        const intx4 v = *(const intx4*)(box + r * ld + c);
-        const float t = sa[r];
-        const float y[4] = {i8_value(p, v[0], t, s.x, b.x), i8_value(p, v[1], t, s.y, b.y), i8_value(p, v[2], t, s.z, b.z), i8_value(p, v[3], t, s.w, b.w)};
-        i8_store4(p, (size_t)(m + r) * p.ldy + n + c, min(4, cols - c), y);
-    }
+    // (asked once for all: a test of each product in the loop costs 3 % of 2500 x 5001 x 1999)
+    bool ordinary = i8_ordinary(sa[lane & 31]);
+#pragma unroll
+    for (int c = 0; c < COLS; c += 64) ordinary = ordinary && i8_ordinary(sw[c + (COLS < 64 ? lane & (COLS - 1) : lane)]);
+    if (__all(ordinary)) i8_rows_out<COLS, true>(p, box, ld, m, n, rows, cols, sa, sw, bias, lane);
+    else i8_rows_out<COLS, false>(p, box, ld, m, n, rows, cols, sa, sw, bias, lane);
 }
 
 // the last `valid` (1..15, or more: all) of a lane's 16 codes of the K dimension stay
@@ -450,10 +476,10 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
     intx4 acc = {0, 0, 0, 0};
     for (int s = 0; s < slices; ++s) acc += *(const intx4*)(p.partial + ((size_t)s * p.M + m) * (quads * 4) + n);
-    const float sa = p.sa[m];
-    float y[4];
+    float y[4], sw[4], bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = i8_value(p, acc[j], sa, i8_channel(p.sw, n + j, p.N), i8_channel(p.bias, n + j, p.N));
+    for (int j = 0; j < 4; ++j) { sw[j] = i8_channel(p.sw, n + j, p.N); bias[j] = i8_channel(p.bias, n + j, p.N); }
+    i8_values<false>(p, acc, p.sa[m], sw, bias, y);
     i8_store4(p, (size_t)m * p.ldy + n, min(4, p.N - n), y);
 }
 
@@ -586,10 +612,10 @@ __global__ void __launch_bounds__(I8_STRIP_THREADS) gemm_i8_strip_kernel(const I
         intx4 v = part[0][f][l];
 #pragma unroll
         for (int u = 1; u < I8_STRIP_WAVES; ++u) v += part[u][f][l];
-        const float sa = TOKENS ? token_scale[m] : p.sa[m];
-        float y[4];
+        float y[4], sw[4], bias[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = i8_value(p, v[e], sa, i8_channel(p.sw, n + e, p.N), i8_channel(p.bias, n + e, p.N));
+        for (int e = 0; e < 4; ++e) { sw[e] = i8_channel(p.sw, n + e, p.N); bias[e] = i8_channel(p.bias, n + e, p.N); }
+        i8_values<false>(p, v, TOKENS ? token_scale[m] : p.sa[m], sw, bias, y);
         i8_store4(p, (size_t)m * p.ldy + n, min(4, p.N - n), y);
     }
 }
