@@ -4,12 +4,14 @@
 #include <cstddef>
 #include <cstdint>
 #include <map>
+#include <set>
 #include <utility>
 
 struct Dim3 { uint32_t x, y, z; };
 
 static int g_device = 0, g_version = 70000000, g_refuse_attribute = 0, g_last = 0;
 static std::map<std::pair<int, const void*>, int> g_limit;          // (device, kernel) -> dynamic shared memory that it may ask for
+static std::set<const void*> g_kernels;                              // launched since the last reset
 static int64_t g_launches = 0, g_attributes = 0, g_threads = 0, g_workgroups = 0;
 static thread_local struct { Dim3 grid, block; size_t shared; void* stream; } t_call;
 
@@ -17,6 +19,8 @@ extern "C" {
 void stand_in_device(int d) { g_device = d; }
 void stand_in_version(int v) { g_version = v; }
 void stand_in_refuse_attribute(int on) { g_refuse_attribute = on; }
+int64_t stand_in_kernels() { return (int64_t)g_kernels.size(); }
+void stand_in_reset_kernels() { g_kernels.clear(); }
 int64_t stand_in_launches() { return g_launches; }
 int64_t stand_in_attributes() { return g_attributes; }
 int64_t stand_in_workgroups() { return g_workgroups; }              // of all launches
@@ -44,6 +48,7 @@ int hipLaunchKernel(const void* f, Dim3 grid, Dim3 block, void**, size_t shared,
     if (shared > 65536 && (it == g_limit.end() || it->second < (int)shared)) return g_last = 1;      // the limit was not raised on this device
     if (threads >= (int64_t)1 << 32 || grid.y > 65535 || grid.z > 65535) return g_last = 9;         // no such configuration
     ++g_launches;
+    g_kernels.insert(f);
     g_workgroups += (int64_t)grid.x * grid.y * grid.z;
     return 0;
 }

@@ -12,7 +12,7 @@ HEAD = """
 import ctypes as C, sys
 hip = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
 lib = C.CDLL(sys.argv[2])
-for n in ("launches", "attributes", "workgroups", "most_threads"):
+for n in ("kernels", "launches", "attributes", "workgroups", "most_threads"):
     getattr(hip, "stand_in_" + n).restype = C.c_int64
 lib.fbhip_last_error.restype = C.c_char_p
 P, L, I = C.c_void_p, C.c_int64, C.c_int32
@@ -79,3 +79,22 @@ for size in SIZES:
     hip.stand_in_refuse_attribute(0)
     assert gemm(*size) == 0
 """)
+
+
+def test_the_sizes_of_the_gpu_tests_reach_every_kernel_of_the_product(run):
+    """as many kernels as a sweep over all sizes launches"""
+    from tests.test_gemm_i8_variants_gpu import SIZES
+    out = run(GEMM + f"""
+for size in {SIZES}:
+    assert gemm(*size) == 0, size
+print(hip.stand_in_kernels())
+hip.stand_in_reset_kernels()
+steps = [1, 2, 16, 17, 32, 33, 64, 65, 100, 200, 400, 800, 1600, 2400, 3200, 5000, 8191, 8192, 8193, 20000]
+for M in steps:
+    for N in steps:
+        for K in (1, 100, 128, 129, 1000, 4096, 5000, 16384, 16385, 131071):
+            assert gemm(M, N, K) == 0, (M, N, K)
+print(hip.stand_in_kernels())
+""")
+    here, everywhere = map(int, out.split())
+    assert here == everywhere == 10, out          # five strips, four tiles, the sum over slices of K
