@@ -1360,11 +1360,17 @@ int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, cons
 }
 
 // ---- products in 8-bit integers --------------------------------------------------------------------------------
+// sizes that the launches' 32-bit arithmetic and their limits of threads hold
+static bool i8_sizes(int M, int N, int K) {
+    constexpr int MOST = 1 << 30;
+    return M >= 1 && N >= 1 && K >= 1 && K <= FBHIP_I8_MAX_K && M <= MOST && N <= MOST && (int64_t)M * (((int64_t)N + 3) / 4) <= (int64_t)255 << 30;
+}
+
 static int check_i8(const char* who, const void* x, const int8_t* w, int64_t ldw, const float* w_scale, const void* y, int64_t ldy, int y_type,
                     int M, int N, int K, const void* workspace, size_t need) {
     if (!x || !w || !w_scale || !y || M < 1 || N < 1 || K < 1) { g_err = std::string(who) + ": an operand is missing or a size is below 1"; return FBHIP_E_INVALID; }
     if (K > FBHIP_I8_MAX_K) { g_err = std::string(who) + ": K > FBHIP_I8_MAX_K: the 32-bit sums could overflow"; return FBHIP_E_INVALID; }
-    if ((int64_t)M * (((int64_t)N + 3) / 4) > (int64_t)255 << 30) { g_err = std::string(who) + ": M * N too large"; return FBHIP_E_INVALID; }
+    if (!i8_sizes(M, N, K)) { g_err = std::string(who) + ": M, N or M * N too large"; return FBHIP_E_INVALID; }
     if (((uintptr_t)w & 15) || (ldw & 15) || ldw < K || ldw > (int64_t)1 << 23) { g_err = std::string(who) + ": weight rows on 16-byte boundaries, K <= ldw <= 2^23 expected"; return FBHIP_E_INVALID; }
     if (ldy < N || y_type < FBHIP_F32 || y_type > FBHIP_F16) { g_err = std::string(who) + ": ldy < N or unknown output type"; return FBHIP_E_INVALID; }
     if (need && (!workspace || ((uintptr_t)workspace & 15))) { g_err = std::string(who) + ": workspace missing or not 16-byte aligned"; return FBHIP_E_INVALID; }
@@ -1384,7 +1390,7 @@ int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* code
 }
 
 size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K) {
-    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K) return 0;
+    if (!i8_sizes(M, N, K)) return 0;
     const I8Plan plan = gemm_i8_plan(M, N, K);
     return plan.slices > 1 ? (size_t)plan.slices * M * (((size_t)N + 3) / 4) * 16 : 0;
 }
@@ -1406,7 +1412,7 @@ static void i8_carve(int M, int K, size_t* scale_at, size_t* rest_at) {
 }
 
 size_t fbhip_linear_i8_workspace(int32_t M, int32_t N, int32_t K) {
-    if (M < 1 || N < 1 || K < 1 || K > FBHIP_I8_MAX_K || linear_i8_fused(M, K)) return 0;
+    if (!i8_sizes(M, N, K) || linear_i8_fused(M, N, K)) return 0;
     size_t scale_at, rest_at;
     i8_carve(M, K, &scale_at, &rest_at);
     return rest_at + fbhip_gemm_i8_workspace(M, N, K);
@@ -1417,7 +1423,7 @@ int fbhip_linear_i8(const void* x, int64_t ldx, int32_t x_type, const int8_t* w,
     fbhip_ctx* none = nullptr;
     RC(check_i8("fbhip_linear_i8", x, w, ldw, w_scale, y, ldy, y_type, M, N, K, workspace, 0));
     if (ldx < K || x_type < FBHIP_F32 || x_type > FBHIP_F16) { g_err = "fbhip_linear_i8: ldx < K or unknown input type"; return FBHIP_E_INVALID; }
-    if (linear_i8_fused(M, K)) {
+    if (linear_i8_fused(M, N, K)) {
         I8Problem p{nullptr, w, nullptr, w_scale, bias, y, nullptr, M, N, K, y_type, relu, 0, 0, ldw, ldy};
         HIPCK(none, launch_linear_i8_tokens(p, x, ldx, x_type, (hipStream_t)stream));
         return FBHIP_OK;

@@ -170,7 +170,7 @@ static void launch_quantize_reg(const void* x, int64_t ldx, int type, int8_t* q,
     else hipLaunchKernelGGL((quantize_rows_reg_kernel<TPR, C, false>), grid, dim3(256), 0, s, x, ldx, type, q, ldq, scale, rows, K, Kp);
 }
 
-hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s) {
+static void launch_quantize_some(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s) {
     const int V = type == FBHIP_F32 ? 4 : 8, pieces = (Kp + V - 1) / V;
     const bool even = ((uintptr_t)q & 7) == 0 && ldq % 8 == 0 && Kp % 8 == 0;          // the codes' rows take whole pieces
     // a wave for a row while a row fits, unless the rows are so few that more threads a row fill the CUs sooner
@@ -180,6 +180,13 @@ hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q,
     else if (even && pieces <= 256 * 4) launch_quantize_reg<256, 4>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
     else if (even && pieces <= 256 * 8) launch_quantize_reg<256, 8>(x, ldx, type, q, ldq, scale, rows, K, Kp, s);
     else hipLaunchKernelGGL(quantize_rows_kernel, dim3(rows), dim3(256), 0, s, x, ldx, type, q, ldq, scale, K, Kp);
+}
+
+hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s) {
+    constexpr int MOST = 1 << 23;                         // rows of a launch, which may have 2^32 - 1 threads
+    for (int64_t r = 0; r < rows; r += MOST)
+        launch_quantize_some((const char*)x + r * ldx * (type == FBHIP_F32 ? 4 : 2), ldx, type, q + r * ldq, ldq, scale + r, (int)std::min<int64_t>(MOST, rows - r),
+                             K, Kp, s);
     return hipGetLastError();
 }
 
@@ -489,6 +496,7 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
 // instructions' share: the operands agree on the order of K, which is all that the sum asks for).  The eight partial sums are added in shared memory.
 // Measured from codes, back to back (us): 5 tokens 1024 x 1024 3.1, 4096 x 4096 5.3, 8192 x 8192 13.6 (67 MB of weights, 4.9 TB/s).
 // TOKENS > 0: up to that many tokens are quantised by every workgroup for itself, while its first weights are on their way: a launch less.
+constexpr int I8_STRIP_MOST = 1 << 26;                    // channels of a launch of strips, which may have 2^32 - 1 threads (tiles take more)
 constexpr int I8_STRIP_WAVES = 8, I8_STRIP_THREADS = 64 * I8_STRIP_WAVES, I8_STRIP_VALUES = 32;      // values of x that a thread holds
 
 // TOKENS rows of x into codes [TOKENS][Kp] and scales in shared memory; 512 / TOKENS threads a row, I8_STRIP_VALUES values a thread
@@ -656,7 +664,7 @@ I8Plan gemm_i8_plan(int M, int N, int K) {
     plan.slices = 1;
     plan.steps = steps;
     const bool long_k = K > 16384 && N < 2048;
-    if (!long_k && (M <= 16 || (M <= 64 && (int64_t)N * K <= (int64_t)1 << 25))) { plan.tile = 16; return plan; }
+    if (!long_k && N <= I8_STRIP_MOST && (M <= 16 || (M <= 64 && (int64_t)N * K <= (int64_t)1 << 25))) { plan.tile = 16; return plan; }
     const int64_t t256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256), t128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
     const int64_t t64 = (int64_t)((M + 63) / 64) * ((N + 63) / 64);
     if (t256 >= 192) plan.tile = 256;
@@ -681,7 +689,7 @@ static void launch_i8_strip(const I8Problem& p, hipStream_t s) {
 // thread more of them fit, but 4 tokens of 8192 values took 29 us in one launch and 18 in two.
 static int i8_tokens(int M) { return M <= 2 ? M : M <= 4 ? 4 : M <= 8 ? 8 : 16; }
 
-bool linear_i8_fused(int M, int K) { return M <= 16 && K <= I8_STRIP_VALUES * I8_STRIP_THREADS / i8_tokens(M); }
+bool linear_i8_fused(int M, int N, int K) { return M <= 16 && N <= I8_STRIP_MOST && K <= I8_STRIP_VALUES * I8_STRIP_THREADS / i8_tokens(M); }
 
 template <int TOKENS>
 static hipError_t launch_i8_strip_tokens(const I8Problem& p, const void* x, int64_t ldx, int xtype, hipStream_t s) {

@@ -213,7 +213,7 @@ struct I8Problem {
 struct I8Plan { int tile, slices, steps, deep; };
 I8Plan gemm_i8_plan(int M, int N, int K);
 hipError_t launch_quantize_rows(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale, int rows, int K, int Kp, hipStream_t s);
-bool linear_i8_fused(int M, int K);          // the tokens are quantised by the product's own launch
+bool linear_i8_fused(int M, int N, int K);          // the tokens are quantised by the product's own launch
 hipError_t launch_linear_i8_tokens(I8Problem p, const void* x, int64_t ldx, int xtype, hipStream_t s);
 hipError_t launch_gemm_i8(I8Problem p, int* partial, hipStream_t s);
 

@@ -78,3 +78,31 @@ def test_quantised_on_the_way(K, M, N, Kd, dtype):
     bias = torch.randn(N, generator=gen, device="cuda")
     q, s = K.quantize_rows(x)
     assert torch.equal(K.linear_i8(x, w, sw, bias=bias, relu=True), K.gemm_i8(q, s, w, sw, bias=bias, relu=True, out_dtype=dtype))
+
+
+def test_more_rows_than_one_launch_takes(K):
+    """2^26 + 5 rows of three values: a wave for each would be 2^32 threads and more"""
+    rows = (1 << 26) + 5
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, 3, generator=gen, device="cuda")
+    q, s = K.quantize_rows(x)
+    assert torch.equal(s, x.abs().amax(1) * torch.tensor(1 / 127, device="cuda"))
+    full = q.as_strided((rows, 128), (128, 1))
+    for r in [0, rows - 1000] + [k * (1 << 23) - 500 for k in range(1, 9)]:
+        some, t = K.quantize_rows(x[r:r + 1000])
+        assert torch.equal(full[r:r + 1000], some.as_strided((len(some), 128), (128, 1))) and torch.equal(s[r:r + 1000], t), r
+    assert bool((full[:, :3].abs().amax(1) == 127).all())
+
+
+@pytest.mark.parametrize("M", [1, 16, 40])
+def test_more_channels_than_a_launch_of_strips_takes(K, M):
+    N = (1 << 26) + 1
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    w = _codes(gen, N, 16)
+    sw = torch.rand(N, generator=gen, device="cuda")
+    x = torch.randn(M, 16, generator=gen, device="cuda")
+    q, s = K.quantize_rows(x)
+    y = K.linear_i8(x, w, sw)
+    assert torch.equal(K.gemm_i8(q, s, w, sw), y)
+    for n in (0, 1 << 25, N - 5000):
+        assert _bad(y[:, n:n + 5000], _sums(q, w[n:n + 5000]), s, sw[n:n + 5000], None, False) == 0

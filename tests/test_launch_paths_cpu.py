@@ -98,3 +98,36 @@ print(hip.stand_in_kernels())
 """)
     here, everywhere = map(int, out.split())
     assert here == everywhere == 10, out          # five strips, four tiles, the sum over slices of K
+
+
+def test_no_launch_has_more_threads_than_one_may(run):
+    """2^32 of them: 67 million short rows to quantise, a hundred million channels, long rows by the million"""
+    run(GEMM + """
+def quantise(rows, K, kind):
+    Kp = -(-K // 128) * 128
+    return lib.fbhip_quantize_rows(P(4096), L(K), I(kind), P(4096), L(Kp), P(4096), I(rows), I(K), I(Kp), None)
+def linear(M, N, K):
+    ld = -(-K // 16) * 16
+    return lib.fbhip_linear_i8(P(4096), L(K), I(0), P(4096), L(ld), P(4096), None, I(0), P(4096), L(N), I(0), I(M), I(N), I(K), P(4096), None)
+for rows, K in ((1 << 26, 3), ((1 << 26) + 5, 3), ((1 << 31) - 1, 3), (1 << 24, 1100), (1 << 24, 30000), ((1 << 23) + 1, 700)):
+    for kind in (0, 1):
+        assert quantise(rows, K, kind) == 0, (rows, K, kind, lib.fbhip_last_error(None))
+for N in ((1 << 26) + 1, 1 << 27, 1 << 28, 1 << 30):
+    for M in (1, 16, 40, 64, 200):
+        assert gemm(M, N, 16) == 0, (M, N)
+        assert linear(M, N, 16) == 0, (M, N)
+assert hip.stand_in_most_threads() < 1 << 32
+for M, N in ((1, (1 << 30) + 1), ((1 << 31) - 1, 1), (1, (1 << 31) - 1)):          # refused, not wrapped
+    assert gemm(M, N, 16) == -1 and linear(M, N, 16) == -1 and b"too large" in lib.fbhip_last_error(None)
+""")
+
+
+def test_rows_of_every_piece_are_quantised_once(run):
+    """the workgroups of all launches are those that the rows need"""
+    out = run("""
+for rows in (1, 4, 5, (1 << 23) - 1, 1 << 23, (1 << 23) + 1, (1 << 26) + 5):
+    before = hip.stand_in_workgroups()
+    assert lib.fbhip_quantize_rows(P(4096), L(3), I(0), P(4096), L(128), P(4096), I(rows), I(3), I(128), None) == 0
+    print(hip.stand_in_workgroups() - before - -(-rows // 4))
+""")
+    assert out.split() == ["0"] * 7, out
