@@ -1385,6 +1385,7 @@ int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* code
     if (!x || !codes || !scale || rows < 1 || K < 1 || Kp < K || ldx < K || ldq < Kp || x_type < FBHIP_F32 || x_type > FBHIP_F16) {
         g_err = "fbhip_quantize_rows: bad argument"; return FBHIP_E_INVALID;
     }
+    if (Kp > INT32_MAX - 1023) { g_err = "fbhip_quantize_rows: K too large: a step along the row would leave 32 bits"; return FBHIP_E_INVALID; }
     HIPCK(none, launch_quantize_rows(x, ldx, x_type, codes, ldq, scale, rows, K, Kp, (hipStream_t)stream));
     return FBHIP_OK;
 }

@@ -204,6 +204,7 @@ def actor_head_bwd(dt1, lnY, lnX, lnStats, lnGamma, W1a, mu, W4, P):
 
 # ------------------------------------------------------------------------------------------------------ products in 8-bit integers
 _TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MOST = 2 ** 31 - 1024          # rows and columns that the entry points and the kernels' steps along a row count in 32 bits
 _checked_devices: tp.Set[int] = set()
 
 
@@ -223,6 +224,8 @@ def _float_rows(x: torch.Tensor, name: str) -> tp.Tuple[int, int, int, int]:
     if x.dim() != 2 or x.dtype not in _TYPE_CODE or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"{name}: a float32, bfloat16 or float16 matrix with contiguous rows expected, got {x.dtype} {tuple(x.shape)} strides {x.stride()}")
     rows, K = x.shape
+    if rows > _MOST or K > _MOST:
+        raise ValueError(f"{name}: at most {_MOST} rows and columns, got {tuple(x.shape)}")
     ld = x.stride(0) if rows > 1 else max(K, 1)
     if ld < K:
         raise ValueError(f"{name}: rows overlap (stride {ld} for {K} columns)")
@@ -234,6 +237,8 @@ def _code_rows(q: torch.Tensor, scale: torch.Tensor, name: str) -> tp.Tuple[int,
     if q.dim() != 2 or q.dtype != torch.int8 or (q.shape[1] > 1 and q.stride(1) != 1):
         raise ValueError(f"{name}: an int8 matrix with contiguous rows expected, got {q.dtype} {tuple(q.shape)} strides {q.stride()}")
     rows, K = q.shape
+    if rows > _MOST or K > _MOST:
+        raise ValueError(f"{name}: at most {_MOST} rows and columns, got {tuple(q.shape)}")
     K16 = (K + 15) // 16 * 16
     ld = q.stride(0) if rows > 1 else K16
     if q.numel() and (ld % 16 or ld < K or q.data_ptr() % 16 or
