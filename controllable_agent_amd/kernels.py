@@ -249,10 +249,24 @@ def _code_rows(q: torch.Tensor, scale: torch.Tensor, name: str) -> tp.Tuple[int,
     return rows, K, ld
 
 
-def _bytes_of(t: torch.Tensor) -> tp.Tuple[int, int]:
-    """first and last byte (exclusive) of a matrix or vector with contiguous rows"""
-    last = (t.shape[0] - 1) * t.stride(0) + (t.shape[1] if t.dim() == 2 else 1) if t.numel() else 0
-    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+def _bytes_of(t: torch.Tensor) -> tp.Tuple[int, int, int, int]:
+    """first and last byte (exclusive) of a matrix or vector with contiguous rows, the bytes of a row and from one row to the next (0: one row)"""
+    rows, cols = (t.shape if t.dim() == 2 else (1, t.shape[0])) if t.numel() else (1, 0)
+    step = t.stride(0) if rows > 1 else 0
+    size = t.element_size()
+    return t.data_ptr(), t.data_ptr() + ((rows - 1) * step + cols) * size, cols * size, step * size
+
+
+def _share_memory(t: torch.Tensor, u: torch.Tensor) -> bool:
+    first, last, row, step = _bytes_of(t)
+    first2, last2, row2, step2 = _bytes_of(u)
+    if first2 >= last or first >= last2:
+        return False
+    if step and step2 and step != step2:          # (rows that lie differently are not followed)
+        return True
+    step = step or step2
+    away = (first2 - first) % step if step else 0
+    return away < row or away + row2 > step       # columns of their own, in rows that lie alike
 
 
 def _i8_output(out, out_dtype, M, N, device, bias, inputs):
@@ -266,10 +280,8 @@ def _i8_output(out, out_dtype, M, N, device, bias, inputs):
     rows, cols, ld, _ = _float_rows(out, "out")
     if (rows, cols) != (M, N) or out.device != device:
         raise ValueError(f"out: [{M}, {N}] on {device} expected, got {tuple(out.shape)} on {out.device}")
-    first, last = _bytes_of(out)
     for t in inputs + (() if bias is None else (bias,)):
-        a, b = _bytes_of(t)
-        if a < last and first < b:
+        if _share_memory(out, t):
             raise ValueError("out: shares memory with an input")
     return out, ld
 

@@ -106,3 +106,17 @@ def test_more_channels_than_a_launch_of_strips_takes(K, M):
     assert torch.equal(K.gemm_i8(q, s, w, sw), y)
     for n in (0, 1 << 25, N - 5000):
         assert _bad(y[:, n:n + 5000], _sums(q, w[n:n + 5000]), s, sw[n:n + 5000], None, False) == 0
+
+
+@pytest.mark.parametrize("M,N,Kd", [(1, 64, 100), (16, 64, 1000), (40, 64, 1024), (300, 200, 500), (2500, 1301, 333)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_answer_beside_its_input(K, M, N, Kd, dtype):
+    """input and output are columns of one buffer, as a layer that hands on both wants them"""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    w, sw = K.quantize_rows(torch.randn(N, Kd, generator=gen, device="cuda"))
+    for before in (0, N):
+        buf = torch.randn(M, Kd + N, generator=gen, device="cuda").to(dtype)
+        x, out = buf[:, before:before + Kd], (buf[:, Kd:] if before == 0 else buf[:, :N])
+        was = x.clone()
+        want = K.linear_i8(x, w, sw)
+        assert K.linear_i8(x, w, sw, out=out) is out and torch.equal(out, want) and torch.equal(x, was)
