@@ -328,18 +328,35 @@ def gemm_i8(A: torch.Tensor, a_scale: torch.Tensor, B: torch.Tensor, b_scale: to
     return C
 
 
+class _Codes(torch.autograd.Function):
+    """hands ``y`` on; a backward pass that asks for the gradient of ``x`` hears that there is none"""
+
+    @staticmethod
+    def forward(ctx, y, x):  # noqa: D102
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, g):  # noqa: D102
+        raise RuntimeError("linear_i8: no gradient flows through 8-bit codes (it is for answers): call it on x.detach() or under torch.no_grad()")
+
+
 def linear_i8(x: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, *, bias: tp.Optional[torch.Tensor] = None, relu: bool = False,
               out_dtype: tp.Optional[torch.dtype] = None, out: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x W^T + bias) with x quantised row by row on the way: ``gemm_i8(*quantize_rows(x), W, w_scale, ...)`` in one call.
 
     x: float32, bfloat16 or float16 [M, K] with contiguous rows; W, w_scale: ``quantize_rows`` of the [N, K] weights; the output has x's type
-    unless ``out_dtype`` or ``out`` says otherwise.  For answers, not for training: no gradient flows through the codes.
+    unless ``out_dtype`` or ``out`` says otherwise.  For answers, not for training: no gradient flows through the codes.  Where ``x`` requires one, a
+    backward pass through the result raises, and ``out`` is refused.
     """
     M, K, ldx, code = _float_rows(x, "x")
     N, K2, ldw = _code_rows(W, w_scale, "W")
     if K != K2 or x.device != W.device:
         raise ValueError(f"x {tuple(x.shape)} on {x.device} and W {tuple(W.shape)} on {W.device} do not go together")
     stream = _stream_on(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("linear_i8: out does not go with an x that requires a gradient: call it on x.detach() or under torch.no_grad()")
+        return _Codes.apply(linear_i8(x.detach(), W, w_scale, bias=bias, relu=relu, out_dtype=out_dtype), x)
     y, ldy = _i8_output(out, x.dtype if out_dtype is None else out_dtype, M, N, x.device, bias, (x, W, w_scale))
     if M == 0 or N == 0:
         return y
