@@ -258,11 +258,18 @@ class AdamW:
         missing = sorted((set(mine) | {"step", "seed"}) - set(state))
         if missing:
             raise ValueError(f"AdamW.load_state_dict: {missing} missing (a state of {self.state_bits} bits expected)")
-        for n, t in mine.items():
-            if state[n].shape != t.shape or state[n].dtype != t.dtype:
-                raise ValueError(f"AdamW.load_state_dict: {n} is {state[n].dtype} {tuple(state[n].shape)}, {t.dtype} {tuple(t.shape)} expected")
+        for n, t in mine.items():          # (everything is looked at before anything is changed)
+            if not isinstance(state[n], torch.Tensor) or state[n].shape != t.shape or state[n].dtype != t.dtype:
+                got = f"{state[n].dtype} {tuple(state[n].shape)}" if isinstance(state[n], torch.Tensor) else type(state[n]).__name__
+                raise ValueError(f"AdamW.load_state_dict: {n} is {got}, {t.dtype} {tuple(t.shape)} expected")
+        try:
+            step, seed = int(state["step"]), int(state["seed"])
+            whole = step == state["step"] and seed == state["seed"] and 0 <= step < 2 ** 63
+        except (TypeError, ValueError, OverflowError):
+            whole = False
+        if not whole:
+            raise ValueError(f"AdamW.load_state_dict: a step count and a seed expected, got {state['step']!r} and {state['seed']!r}")
         for n, t in mine.items():
             t.copy_(state[n])
-        self.seed = int(state["seed"]) & 0xFFFFFFFF
-        self._opt.seed = self.seed
-        self._set_step(int(state["step"]))
+        self.seed = self._opt.seed = seed & 0xFFFFFFFF
+        self._set_step(step)

@@ -62,3 +62,20 @@ def test_matrices_with_rows_apart():
         with pytest.raises(ValueError):
             opt._grad_types([bad])
         assert opt._grad_types([torch.zeros(8, 12)[:, :6]]) == b"\0"
+
+
+@pytest.mark.parametrize("change", [dict(step=-1), dict(step=2.5), dict(step=None), dict(step=2 ** 63), dict(seed="x"), dict(m=[1.0]), dict(v=torch.zeros(256).double()),
+                                    dict(v=torch.zeros(512))], ids=str)
+def test_a_state_that_is_refused_leaves_everything_as_it_was(change):
+    opt = object.__new__(AdamW)
+    opt.state_bits, opt.seed = 32, 7
+    opt.m, opt.v = torch.zeros(256), torch.zeros(256)
+    steps = []
+    opt._set_step = steps.append
+    opt._opt = type("Opt", (), {"seed": 7})()
+    with pytest.raises(ValueError):
+        opt.load_state_dict({**dict(m=torch.ones(256), v=torch.ones(256), step=3, seed=9), **change})
+    assert not steps and not opt.m.any() and not opt.v.any() and opt.seed == opt._opt.seed == 7
+    for step in (3, 3.0, torch.tensor(3), torch.tensor(3.0)):
+        opt.load_state_dict(dict(m=torch.ones(256), v=torch.ones(256), step=step, seed=9))
+    assert steps == [3] * 4 and opt.m.all() and opt.v.all() and opt.seed == opt._opt.seed == 9
