@@ -158,10 +158,11 @@ class AdamW:
     def _interleaved(self, i: int, j: int) -> bool:
         (ci, li), (cj, lj) = self._layouts[i], self._layouts[j]
         p, q = self.params[i], self.params[j]
-        if not (ci and cj and li == lj and p.dtype == q.dtype):
+        ld = li or lj                              # (what is dense is one row among the other's)
+        if not ld or (li and lj and li != lj) or p.dtype != q.dtype:
             return False
-        away = (q.data_ptr() - p.data_ptr()) // p.element_size() % li
-        return away >= ci and away + cj <= li
+        away = (q.data_ptr() - p.data_ptr()) // p.element_size() % ld
+        return away >= (ci or p.numel()) and away + (cj or q.numel()) <= ld
 
     def _set_step(self, step: int) -> None:
         with torch.cuda.device(self.device):

@@ -79,3 +79,14 @@ def test_a_state_that_is_refused_leaves_everything_as_it_was(change):
     for step in (3, 3.0, torch.tensor(3), torch.tensor(3.0)):
         opt.load_state_dict(dict(m=torch.ones(256), v=torch.ones(256), step=step, seed=9))
     assert steps == [3] * 4 and opt.m.all() and opt.v.all() and opt.seed == opt._opt.seed == 9
+
+
+def test_a_row_beside_the_columns_of_the_others():
+    """one row of a matrix is dense; it shares no memory with other columns of the same matrix"""
+    buf = torch.zeros(10, 10)
+    for params in ([buf[1:2, :5], buf[:, 5:]], [buf[:, :5], buf[3, 5:]], [buf[:, 3:5], buf[3, 5:], buf[4, :3], buf[5:6, 5:9]]):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            AdamW(params)
+    for params in ([buf[1:2, :6], buf[:, 5:]], [buf[:, :5], buf[3, 4:]], [buf[:, :5], buf.view(-1)[35:46]], [buf[1], buf[:, 5:]], [buf[0, :3], buf[0, 2:5]]):
+        with pytest.raises(ValueError, match="share memory"):
+            AdamW(params)
