@@ -107,3 +107,35 @@ def test_a_second_step_refuses_what_a_first_one_does(AdamW):
     assert opt.step_count == 1 and torch.equal(p, before)
     opt.step([torch.ones(4, 6, device="cuda", dtype=torch.float16)])
     assert opt.step_count == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_agents_own_networks(AdamW, bits):
+    """the rows of a NetView's matrices are padded in one flat buffer: a step moves what belongs to the network, bit for bit, and leaves the padding zero and
+    the other networks as they were; gradients with the parameters' strides, or dense"""
+    from oracle import fb_oracle as fo
+    from tests import helpers as H
+    cfg = fo.OracleConfig(obs_dim=5, action_dim=3, goal_dim=5, z_dim=10, hidden_dim=36, feature_dim=16, backward_hidden_dim=22, batch_size=32)
+    rng = np.random.default_rng(4)
+    agent = H.make_hip_agent(cfg, {n: fo.synthetic_params(rng, fo.NET_SHAPES[n](cfg)) for n in ("actor", "forward_net", "backward_net")})
+    params = list(agent.forward_net.parameters()) + list(agent.backward_net.parameters())
+    assert any(not p.is_contiguous() for p in params) and all(p.is_cuda for p in params)
+    others = {n: {k: v.clone() for k, v in getattr(agent, n).state_dict().items()} for n in ("actor", "forward_target_net", "backward_target_net")}
+    lr, b1, b2, eps, wd = 1e-3, 0.9, 0.999, 1e-8, 0.01
+    opt = AdamW(params, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, state_bits=bits)
+    P = [p.cpu().numpy().copy() for p in params]
+    gen = torch.Generator().manual_seed(bits)
+    G = [(torch.randn(p.shape, generator=gen) * 1e-2) for p in params]
+    grads = [g.cuda() if k % 2 else torch.empty_strided(p.shape, p.stride(), device="cuda").copy_(g) for k, (g, p) in enumerate(zip(G, params))]
+    opt.step(grads)
+    for k, (p, want, g) in enumerate(zip(params, P, (g.numpy() for g in G))):
+        M = F(0) + F(1 - b1) * (g - F(0))
+        V = F(0) * F(b2) + (F(1 - b2) * g) * g
+        want = want * F(1 - lr * wd) - F(lr / (1 - b1)) * (M / (np.sqrt(V) * F(1 / math.sqrt(1 - b2)) + F(eps)))
+        assert np.array_equal(p.cpu().numpy(), want), k
+        if bits == 32:
+            m, v = (x.cpu().numpy().reshape(p.shape) for x in opt.moments(k))
+            assert np.array_equal(m, M) and np.array_equal(v, V), k
+    assert agent.forward_net.pad_abs_max() == 0 and agent.backward_net.pad_abs_max() == 0 and agent.actor.pad_abs_max() == 0
+    for n, was in others.items():
+        assert all(torch.equal(v, was[k]) for k, v in getattr(agent, n).state_dict().items()), n
