@@ -1,4 +1,4 @@
-"""AdamW over a list of tensors in one launch, moments in 32 or in 8 bits (csrc/adamw.hip).
+"""AdamW over a list of tensors in one launch (384 tensors each), moments in 32 or in 8 bits (csrc/adamw.hip).
 
 ``kernels.adam_ema`` moves one flat fp32 buffer with Adam's fixed settings, as the agents' own networks need it; this is the optimiser for
 everything else a user trains beside them: any number of tensors of any sizes, fp32 or bf16, with decoupled weight decay, clipping by the
@@ -57,7 +57,8 @@ def _per_tensor(name: str, value, n: int) -> tp.List[float]:
 
 
 class AdamW:
-    """``opt = AdamW(params); opt.step(grads)``: p <- (1 - lr wd) p - lr m^ / (sqrt(v^) + eps), all tensors in one launch.
+    """``opt = AdamW(params); opt.step(grads)``: p <- (1 - lr wd) p - lr m^ / (sqrt(v^) + eps), all tensors in one launch (384 of them a launch, and
+    one more each to clip).  Every value is the formulas' chain of correctly rounded single-precision operations.
 
     ``params``: float32 or bfloat16 device tensors, changed in place; dense in any order of dimensions, or row-strided matrices (the
     agents' ``NetView`` entries).  bfloat16 parameters are rounded up or down at random, so that small updates count on average.

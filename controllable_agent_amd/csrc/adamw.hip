@@ -8,11 +8,11 @@
 // written once; a lane holds eight consecutive elements, so that each 16-bit stream is one 16-byte access, an fp32 one two and a code
 // stream one of 8 bytes, and a block of 256 elements that shares a scale is half a wave: its maximum is five lane exchanges.  (Four elements a
 // lane leave room for more waves and take 20 % longer: the accesses are half as wide.)
-// Measured, on a card whose large copy reaches 4.93 TB/s: 134 M fp32 parameters, bf16 gradients, 8-bit moments 422 us (4.47 TB/s, the arithmetic shows);
-// 67 M in bf16 with fp32 moments and their norm 329 us (4.89 TB/s; more loads under way in the norm gained 1 % there and lost 10 % on 3.7 M); 3.7 M in
-// fp32 21 us (32 bits), 23 us (8 bits and the norm), of which the start of a workgroup (scalars, tables, first loads) is a third.
-// Root and quotient are correctly rounded, as the plain form's are.  With the instructions that are good to a step (v_sqrt_f32, v_rcp_f32) these took 380,
-// 325, 21 and 22 us, but parameters differed in their last bit from the formulas' single-precision operations, and now and then a code of r by a step.
+// Measured, on a card whose large copy reaches 4.93 TB/s: 134 M fp32 parameters, bf16 gradients, 8-bit moments 407 us (4.64 TB/s, the arithmetic shows);
+// 67 M in bf16 with fp32 moments and their norm 328 us (4.91 TB/s; more loads under way in the norm gained 1 % there and lost 10 % on 3.7 M); 3.7 M in
+// fp32 21 us (32 bits), 23.5 us (8 bits 19, the norm 4 to 6), of which the start of a workgroup (scalars, tables, first loads) is a third.
+// Root and quotient are correctly rounded, as the plain form's are.  With the instructions that are good to a step (v_sqrt_f32, v_rcp_f32) these took 376,
+// 324, 21 and 21.7 us, but parameters differed in their last bit from the formulas' single-precision operations, and now and then a code of r by a step.
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 codes times a power of two for each 256 elements (the least one under which the
 // block's largest magnitude is at most 448).  r, not v: the step divides by sqrt(v), and the root halves the range that the codes have to
@@ -30,9 +30,10 @@ namespace fbhip {
 constexpr int ADAMW_THREADS = 256, ADAMW_PER_LANE = 8, ADAMW_CHUNK = ADAMW_THREADS * ADAMW_PER_LANE;
 static_assert(ADAMW_CHUNK == FBHIP_ADAMW_CHUNK, "the caller's chunk table counts chunks of this size");
 constexpr int ADAMW_MAX_TENSORS = 384;       // gradient addresses travel in the kernel arguments (4 KB): valid in a captured graph
-// Workgroups that are all on the 256 CUs at once and walk the chunks (2048 of them: the second lot runs on CUs that are half empty, 24.2 and 20.2 us
-// for the walker networks).  With 32-bit moments three a CU keep memory busy, and more of them only spread the accesses: 67 M in bf16 327 us
-// with three, 330 with four, 333 with five.  With 8-bit moments the arithmetic wants all five that the registers allow: 134 M 381 us, 395 with four.
+// Workgroups that are all on the 256 CUs at once and walk the chunks (more of them: the second lot runs on CUs that are half empty; with six a CU the
+// walker networks take 28.0 us with 8-bit moments and clipping, with five 23.7).  With 32-bit moments three a CU keep memory busy, and more of them only
+// spread the accesses: 67 M in bf16 329 us with three, 329 with four, 332 with five.  With 8-bit moments the arithmetic wants all five that the registers
+// allow: 134 M 416 us, 470 with three, 431 with four, 463 with six.
 constexpr int ADAMW_BLOCKS_32 = 3 * 256, ADAMW_BLOCKS_8 = 5 * 256;
 constexpr int ADAMW_NORM_BLOCKS = 1024;      // one partial sum each, folded in order
 
@@ -144,7 +145,8 @@ __device__ __forceinline__ void load_grad(const fbhip_adamw_tensor& T, const voi
     }
 }
 
-// A 32-bit word for an element: its place is multiplied and shifted into the step's key (two rounds of multiply and shift-xor).
+// A 32-bit word for an element: its place is multiplied and shifted into the step's key (two rounds of multiply and shift-xor: the published 32-bit
+// finaliser of MurmurHash3).
 __device__ __forceinline__ uint32_t finish_word(uint32_t h) {
     h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
     h = (h ^ (h >> 13)) * 0xC2B2AE35u;

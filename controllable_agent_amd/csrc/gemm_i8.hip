@@ -102,7 +102,7 @@ __device__ __forceinline__ uint4 i8_piece(const char* base, int k, int K) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Bound by memory: x is read once, the codes are written once (8192^2 bf16: 35 us, 5.8 TB/s, part of it from the Infinity Cache).
+// Bound by memory: x is read once, the codes are written once (8192^2 bf16: 34 us, 6.0 TB/s, part of it from the Infinity Cache).
 // A row in the registers of TPR threads: C pieces of 16 bytes a thread, read once, whatever the row's alignment.
 template <int TPR, int C, bool WIDE>
 __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const void* __restrict__ x, int64_t ldx, int type, int8_t* __restrict__ q, int64_t ldq,
@@ -299,8 +299,9 @@ __device__ __forceinline__ intx4 i8_mask(intx4 v, int valid) {
 // ------------------------------------------------------------------------------------------------------------------ tiles
 // A workgroup of WN x WM waves computes a tile of (WN FN 32) channels x (WM FM 32) tokens; a wave keeps FN x FM accumulators of the
 // 32x32x32 matrix instruction, the weights as its first operand, so that a lane holds four neighbouring channels of one token.
-// Measured from codes, back to back (us, fp32 out): 8192^3 479 (2.30 PTOPS; the clock falls to 1.7 GHz, matrix instructions alone on such
-// operands reach 3.45), 4096^3 66-70 (1.66 a step of 128 and 15 for start and output), 2500 x 5001 x 1999 36-39, 4096 x 2048 x 2048 24, 1024 x 2048 x 1024 8.4.
+// Measured from codes, back to back on one input (us, fp32 out): 8192^3 480 (2.29 PTOPS; the clock falls to 1.7 GHz, matrix instructions alone on such
+// operands reach 3.45), 4096^3 67-70 (1.66 a step of 128 and 15 for start and output), 2500 x 5001 x 1999 37-40, 4096 x 2048 x 2048 24-26,
+// 1024 x 2048 x 1024 8.3.  Inputs in turn and launches apart cost more: 8192^3 with three inputs 500-505, one launch after a pause 532, under a trace 538-566.
 // A step takes BK bytes of K: both operands' rows of it come straight into shared memory (16 bytes a lane), S steps deep.  Shared memory
 // has 64 banks: a fragment read of 16 rows' 16-byte pieces is free of conflicts if rows that lie a multiple of 256 bytes apart keep them in
 // different places, so the pieces of row r are stored in the order piece ^ (r / (256 / BK)).
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(256) gemm_i8_fold_kernel(const I8Problem p, in
 // Few tokens: what counts is the weights' way from memory.  A workgroup of eight waves takes 16 NT channels and up to 16 MT tokens, its waves 128
 // codes of K in turn, both operands straight from memory into the 16x16x64 matrix instruction (a lane's 32 codes in a row are two
 // instructions' share: the operands agree on the order of K, which is all that the sum asks for).  The eight partial sums are added in shared memory.
-// Measured from codes, back to back (us): 5 tokens 1024 x 1024 3.1, 4096 x 4096 5.3, 8192 x 8192 13.6 (67 MB of weights, 4.9 TB/s).
+// Measured from codes, back to back (us): 5 tokens 1024 x 1024 2.8, 4096 x 4096 5.2, 8192 x 8192 14.0 (67 MB of weights, 4.8 TB/s).
 // TOKENS > 0: up to that many tokens are quantised by every workgroup for itself, while its first weights are on their way: a launch less.
 constexpr int I8_STRIP_MOST = 1 << 26;                    // channels of a launch of strips, which may have 2^32 - 1 threads (tiles take more)
 constexpr int I8_STRIP_WAVES = 8, I8_STRIP_THREADS = 64 * I8_STRIP_WAVES, I8_STRIP_VALUES = 32;      // values of x that a thread holds

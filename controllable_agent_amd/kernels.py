@@ -310,7 +310,7 @@ def gemm_i8(A: torch.Tensor, a_scale: torch.Tensor, B: torch.Tensor, b_scale: to
             relu: bool = False, out_dtype: torch.dtype = torch.float32, out: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
     """C[m, n] = act((sum_k A[m, k] B[n, k]) * a_scale[m] * b_scale[n] + bias[n]) on int8 codes A [M, K] (tokens) and B [N, K] (channels).
 
-    The sums are exact (K <= 131071).  Rows lie on 16-byte boundaries and can be read to a multiple of 16, as ``quantize_rows`` makes them.
+    The sums are exact (K <= 131071; M, N <= 2^30).  ``out`` may lie in columns of its own beside an input, but not share memory with one.  Rows lie on 16-byte boundaries and can be read to a multiple of 16, as ``quantize_rows`` makes them.
     """
     M, K, lda = _code_rows(A, a_scale, "A")
     N, K2, ldb = _code_rows(B, b_scale, "B")

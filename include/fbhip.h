@@ -520,11 +520,12 @@ int fbhip_adamw_step(const fbhip_adamw* opt, const void* const* host_grads, cons
 #define FBHIP_I8_MAX_K 131071              /* the int32 sums cannot overflow up to here: 128 * 128 * K < 2^31 */
 /* scale[r] = max|x[r, :]| * (1 / 127 as a float32), codes[r, k] = nearest whole number to x[r, k] / scale[r] (ties to even).  x: FBHIP_F32 / BF16 / F16, rows
  * ldx elements apart.  codes: rows ldq bytes apart, ldq >= Kp; columns K .. Kp - 1 are set to 0.  A row with a NaN or an infinity: scale NaN,
- * codes 0; a row of zeros: scale 0, codes 0. */
+ * codes 0; a row of zeros: scale 0, codes 0.  Kp <= 2^31 - 1024. */
 int fbhip_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int8_t* codes, int64_t ldq, float* scale, int32_t rows, int32_t K,
                         int32_t Kp, void* stream);
 /* y[m, n] = act((sum_k a[m, k] w[n, k]) * a_scale[m] * w_scale[n] + bias[n]).  a, w: 8-bit codes, rows on 16-byte boundaries and readable to the
  * next multiple of 16 (what lies behind K does not count).  bias nullable; relu: 0 / 1; y: FBHIP_F32 / BF16 / F16, rows ldy elements apart.
+ * M, N <= 2^30.  Scales whose product leaves float32's normal range are applied with their exponents apart: a sum of 0 stays 0.
  * workspace: fbhip_gemm_i8_workspace / fbhip_linear_i8_workspace bytes (16-byte aligned; nullable where that is 0). */
 size_t fbhip_gemm_i8_workspace(int32_t M, int32_t N, int32_t K);
 int fbhip_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,

@@ -1,5 +1,5 @@
 """Two REAL ranks of the HIP data-parallel path on one GPU (both on cuda:0, backend gloo -- RCCL refuses two ranks on
-one device, gloo all-reduces CUDA tensors fine): every rank runs FBHipAgent.update on its own replay shard through
+one device; gloo is given host copies): every rank runs FBHipAgent.update on its own replay shard through
 controllable_agent_amd.distributed.dp_update (3 hipGraphs + 2 gradient all-reduces per step).  Must equal ONE process fed
 both micro-batches with gradient averaging (the oracle, as in tests/test_distributed_cpu.py) and leave the replicas
 bit-identical.  This is the rehearsal of the 8-GPU RCCL run the driver does at round end."""
