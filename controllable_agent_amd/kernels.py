@@ -329,11 +329,11 @@ def gemm_i8(A: torch.Tensor, a_scale: torch.Tensor, B: torch.Tensor, b_scale: to
 
 
 class _Codes(torch.autograd.Function):
-    """hands ``y`` on; a backward pass that asks for the gradient of ``x`` hears that there is none"""
+    """``linear_i8`` of an ``x`` that requires a gradient: a backward pass that asks for it hears that there is none"""
 
     @staticmethod
-    def forward(ctx, y, x):  # noqa: D102
-        return y.view_as(y)
+    def forward(ctx, x, W, w_scale, bias, relu, out_dtype):  # noqa: D102
+        return linear_i8(x, W, w_scale, bias=bias, relu=relu, out_dtype=out_dtype)          # (gradients are off in here)
 
     @staticmethod
     def backward(ctx, g):  # noqa: D102
@@ -356,7 +356,7 @@ def linear_i8(x: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, *, bias: 
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("linear_i8: out does not go with an x that requires a gradient: call it on x.detach() or under torch.no_grad()")
-        return _Codes.apply(linear_i8(x.detach(), W, w_scale, bias=bias, relu=relu, out_dtype=out_dtype), x)
+        return _Codes.apply(x, W, w_scale, bias, relu, out_dtype)
     y, ldy = _i8_output(out, x.dtype if out_dtype is None else out_dtype, M, N, x.device, bias, (x, W, w_scale))
     if M == 0 or N == 0:
         return y

@@ -28,3 +28,16 @@ def test_a_backward_pass_through_the_codes_raises(M):
     with torch.no_grad():
         z = K.linear_i8(x, codes, scale, bias=bias, relu=True, out=torch.empty(M, 30, device="cuda"))
     assert torch.equal(z, want) and not z.requires_grad
+
+
+def test_its_result_may_be_changed_in_place():
+    from controllable_agent_amd import kernels as K
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(20, 100, generator=gen).cuda()
+    codes, scale = K.quantize_rows(torch.randn(30, 100, generator=gen).cuda())
+    want = K.linear_i8(x, codes, scale).add_(1).mul_(2)
+    got = K.linear_i8(x.clone().requires_grad_(True), codes, scale).add_(1).mul_(2)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="no gradient flows"):
+        got.sum().backward()
+    assert torch.equal(K.linear_i8(x[:0].requires_grad_(True), codes, scale), torch.zeros(0, 30, device="cuda"))
