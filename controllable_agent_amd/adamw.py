@@ -22,6 +22,7 @@ CHUNK = 2048           # FBHIP_ADAMW_CHUNK
 GRAD_DENSE = 4         # FBHIP_GRAD_DENSE
 CONTROL_BYTES = 2304   # FBHIP_ADAMW_CONTROL_BYTES
 _DTYPE = operator.attrgetter("dtype")
+_FLOAT_MAX = torch.finfo(torch.float32).max
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -218,8 +219,8 @@ class AdamW:
             lr_ptr = lr.data_ptr()
         else:
             lr_value = float(lr)
-        if not (math.isfinite(lr_value) and math.isfinite(grad_scale)):
-            raise ValueError(f"AdamW.step: finite lr and grad_scale expected, got {lr} and {grad_scale}")
+        if not (abs(lr_value) <= _FLOAT_MAX and abs(grad_scale) <= _FLOAT_MAX):
+            raise ValueError(f"AdamW.step: finite lr and grad_scale (in float32) expected, got {lr} and {grad_scale}")
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"AdamW.step: max_norm > 0 expected, got {max_norm}")
         pointers = array.array("Q", map(torch.Tensor.data_ptr, grads))

@@ -90,3 +90,11 @@ def test_a_row_beside_the_columns_of_the_others():
     for params in ([buf[1:2, :6], buf[:, 5:]], [buf[:, :5], buf[3, 4:]], [buf[:, :5], buf.view(-1)[35:46]], [buf[1], buf[:, 5:]], [buf[0, :3], buf[0, 2:5]]):
         with pytest.raises(ValueError, match="share memory"):
             AdamW(params)
+
+
+@pytest.mark.parametrize("kw", [dict(grad_scale=1e39), dict(grad_scale=-1e39), dict(lr=1e39), dict(lr=float("nan")), dict(grad_scale=float("inf")), dict(max_norm=0.0)], ids=str)
+def test_numbers_that_float32_does_not_hold(kw):
+    opt = _checker([torch.zeros(4)])
+    opt.lr = 1e-3
+    with pytest.raises(ValueError):
+        opt.step([torch.zeros(4)], **kw)
